@@ -26,7 +26,7 @@ static thread_local std::string g_err;
 static std::atomic<long long> g_launches{0};  // kernel launches issued so far (fa_b200_launch_count)
 
 static int fail(int code, const std::string& msg);
-int fail_bwd(int code, const std::string& msg) { return fail(code, msg); }  // for bwd.cu
+int fail_bwd(int code, const std::string& msg) { return fail(code, msg); }  // for bwd.cu, kv8_api.cu
 void count_launches(int n) { g_launches += n; }
 static int fail(int code, const std::string& msg) {
   g_err = msg;
@@ -442,6 +442,14 @@ static int launch_combine(const fa_combine_params& c, cudaStream_t st) {
   ++g_launches;
   return FA_OK;
 }
+
+// for kv8_api.cu
+int merge_partials(const fa_combine_params& c, cudaStream_t st) { return launch_combine(c, st); }
+void window_rule(int seqlen_q, int max_k, bool causal, int& wl, int& wr, bool& is_causal, bool& is_local) {
+  normalize_window(seqlen_q, max_k, causal, wl, wr, is_causal, is_local);
+}
+int sm_count() { return device_sm_count(); }
+void clear_error() { g_err.clear(); }
 
 // Device scratch of one call: given by the caller, or asked for once its size is known.
 struct Workspace {

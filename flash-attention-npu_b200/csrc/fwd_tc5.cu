@@ -364,6 +364,18 @@ bool tma_encode_rows(CUtensorMap* m, const void* ptr, int dtype, int d, int head
   return tc5::encode_map(m, ptr, dtype, d, heads, rows, outer, head_stride, row_stride, outer_stride, box_rows);
 }
 
+bool kv8_encode_map(CUtensorMap* m, const void* ptr, int d, int heads, int64_t rows, int64_t outer, int64_t head_stride,
+                    int64_t row_stride, int64_t outer_stride, int box_cols, int box_rows) {
+  tc5::EncodeFn enc = tc5::get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)outer};
+  cuuint64_t strides[3] = {(cuuint64_t)head_stride, (cuuint64_t)row_stride, (cuuint64_t)outer_stride};
+  cuuint32_t box[4] = {(cuuint32_t)box_cols, 1, (cuuint32_t)box_rows, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             box_cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int tc5_read_status(cudaStream_t st) {
   int32_t* w = tc5::status_word();
   if (!w) return 0;

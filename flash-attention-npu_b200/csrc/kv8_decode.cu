@@ -1,0 +1,17 @@
+// Host side of the 8-bit decode kernel: tile facts and tensor maps.
+#include "kv8_api.cuh"
+#include "kv8_decode_kernel.cuh"
+#include "tc5_api.cuh"
+
+namespace fa {
+
+template <class Tr>
+static Kv8TileInfo info() { return Kv8TileInfo{Tr::BM, Tr::BN, Tr::NTHREADS, Tr::SMEM_BYTES, Tr::RESIDENT}; }
+
+Kv8TileInfo kv8_decode_info(int hd, bool wide) {
+  if (hd == 64) return wide ? info<Kv8Traits<64, 2>>() : info<Kv8Traits<64, 1>>();
+  if (hd == 128) return wide ? info<Kv8Traits<128, 2>>() : info<Kv8Traits<128, 1>>();
+  return wide ? info<Kv8Traits<256, 2>>() : info<Kv8Traits<256, 1>>();
+}
+
+}  // namespace fa

@@ -1,0 +1,4 @@
+#define FA_INST_HD 128
+#define FA_INST_CODE FA_CODE_E4M3
+#define FA_INST_NAME launch_kv8_decode_128_e4m3
+#include "kv8_decode_inst.inc"

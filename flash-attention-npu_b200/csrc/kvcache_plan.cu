@@ -1,0 +1,128 @@
+// One serving step's bookkeeping on the GPU: pages for the requests that grow, the slot and position of every new token, packed
+// offsets, lengths afterwards.  Integers only; a host that never learns the lengths can capture the step into a graph.
+//
+// Request r holds ceil(have / page) pages and needs ceil((have + new) / page).  The missing ones come off the free list in request
+// order, so request r's start in the list is a prefix sum; a request whose row of the table or the list has no room is left as it
+// was (the prefix sum goes on as if it had been served, so that the pages taken are always the list's first ones).
+//
+// Latency-bound: a few bytes a token.  One launch: every CTA sums up all requests by itself (two prefix sums of b entries, from L2)
+// and then writes its share of the tokens and of the table, so no CTA waits for another.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace fa {
+
+constexpr int kPlanThreads = 256, kPlanTokens = 4 * kPlanThreads;
+
+struct PlanRequest {
+  int64_t have, add;
+  int had, need;
+  bool fits;
+};
+__device__ __forceinline__ PlanRequest plan_request(const fa_kvcache_plan_params& p, int r) {
+  PlanRequest q;
+  q.have = p.have[r];
+  q.add = p.add[r];
+  q.fits = q.have >= 0 && q.add >= 0 && q.have + q.add <= (int64_t)p.cols * p.page_size;
+  q.add = max(q.add, (int64_t)0);
+  q.had = q.fits ? (int)((q.have + p.page_size - 1) / p.page_size) : 0;
+  q.need = q.fits ? (int)((q.have + q.add + p.page_size - 1) / p.page_size) - q.had : 0;
+  return q;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid_constant__ fa_kvcache_plan_params p, int32_t* status) {
+  extern __shared__ int2 s_pre[];  // per request: tokens and pages in front of it; [b]: of all
+  __shared__ int2 s_warp[kPlanThreads / 32];
+  __shared__ int s_pages;
+  grid_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = ceil_div(p.b, kPlanThreads), r0 = min(p.b, tid * per), r1 = min(p.b, r0 + per);
+  int2 sum = make_int2(0, 0);
+  for (int r = r0; r < r1; ++r) {
+    const PlanRequest q = plan_request(p, r);
+    s_pre[r] = sum;
+    sum.x += (int)q.add;
+    sum.y += q.need;
+  }
+  int2 incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
+    if (lane >= o) { incl.x += x; incl.y += y; }
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  if (tid == 0) s_pages = 0;
+  __syncthreads();
+  int2 base = make_int2(incl.x - sum.x, incl.y - sum.y);
+  for (int w = 0; w < warp; ++w) { base.x += s_warp[w].x; base.y += s_warp[w].y; }
+  for (int r = r0; r < r1; ++r) { s_pre[r].x += base.x; s_pre[r].y += base.y; }
+  if (tid == kPlanThreads - 1) s_pre[p.b] = make_int2(base.x + sum.x, base.y + sum.y);
+  __syncthreads();
+
+  int n_free = p.n_free;
+  if (p.num_free) n_free = min(max(*p.num_free, 0), p.n_free);
+  auto granted = [&](const PlanRequest& q, int r) { return q.fits && (q.need == 0 || s_pre[r].y + q.need <= n_free); };
+  // requests: a warp each
+  const int warps = gridDim.x * (kPlanThreads / 32), gw = blockIdx.x * (kPlanThreads / 32) + warp;
+  for (int r = gw; r < p.b; r += warps) {
+    const PlanRequest q = plan_request(p, r);
+    const bool ok = granted(q, r);
+    if (lane == 0) {
+      p.after[r] = (int)(ok ? q.have + q.add : p.have[r]);
+      p.cu_new[r] = s_pre[r].x;
+      if (!ok && !(q.have >= 0 && p.add[r] >= 0)) raise_bad_index(status);
+    }
+    if (ok)
+      for (int i = lane; i < q.need; i += 32) p.table[(int64_t)r * p.table_stride + q.had + i] = p.free_pages[s_pre[r].y + i];
+  }
+  if (blockIdx.x == 0) {
+    int most = 0;
+    for (int r = tid; r < p.b; r += kPlanThreads) {
+      const PlanRequest q = plan_request(p, r);
+      if (q.need > 0 && granted(q, r)) most = max(most, s_pre[r].y + q.need);
+    }
+    atomicMax(&s_pages, most);
+    __syncthreads();
+    if (tid == 0) {
+      *p.pages_taken = s_pages;
+      p.cu_new[p.b] = s_pre[p.b].x;
+    }
+  }
+  // tokens
+  const int last = s_pre[p.b].x;
+  for (int64_t t = (int64_t)blockIdx.x * kPlanThreads + tid; t < p.total; t += (int64_t)gridDim.x * kPlanThreads) {
+    int64_t slot = -1;
+    int pos = 0;
+    if (t < last) {
+      int lo = 0, hi = p.b;  // the last request that starts at or in front of t (empty ones start where the next does)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_pre[mid].x <= t) lo = mid;
+        else hi = mid;
+      }
+      const PlanRequest q = plan_request(p, lo);
+      const int64_t at = q.have + (t - s_pre[lo].x);
+      pos = (int)at;
+      if (granted(q, lo) && at >= 0 && at < q.have + q.add) {
+        const int col = (int)(at / p.page_size), in = (int)(at - (int64_t)col * p.page_size);
+        const int page = col < q.had ? p.table[(int64_t)lo * p.table_stride + col] : p.free_pages[s_pre[lo].y + col - q.had];
+        slot = (int64_t)page * p.page_size + in;
+      }
+    }
+    p.slots[t] = slot;
+    p.positions[t] = pos;
+  }
+}
+
+cudaError_t launch_kvcache_plan(const fa_kvcache_plan_params& p, int num_sm, int32_t* status, cudaStream_t st) {
+  int64_t grid = (p.total + kPlanTokens - 1) / kPlanTokens;
+  grid = std::max<int64_t>(grid, ceil_div(p.b, 4 * (kPlanThreads / 32)));
+  grid = std::min<int64_t>(std::max<int64_t>(grid, 1), num_sm);
+  const size_t smem = (size_t)(p.b + 1) * sizeof(int2);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kvcache_plan_kernel), (FA_B200_PLAN_MAX_REQUESTS + 1) * (int)sizeof(int2));
+  if (e != cudaSuccess) return e;
+  return launch_dependent(kvcache_plan_kernel, dim3((unsigned)grid), kPlanThreads, smem, st, p, status);
+}
+
+}  // namespace fa

@@ -22,6 +22,9 @@ int tc5_read_status(cudaStream_t st);
 // 64 columns x 1 head x box_rows rows x 1, 128-byte swizzle.  Returns false when the driver refuses.
 bool tma_encode_rows(CUtensorMap* m, const void* ptr, int dtype, int d, int heads, int64_t rows, int64_t outer,
                      int64_t head_stride, int64_t row_stride, int64_t outer_stride, int box_rows);
+// The same over codes of one byte: box = box_cols (64 or 128) columns x 1 head x box_rows rows x 1, swizzled over box_cols bytes.
+bool kv8_encode_map(CUtensorMap* m, const void* ptr, int d, int heads, int64_t rows, int64_t outer, int64_t head_stride,
+                    int64_t row_stride, int64_t outer_stride, int box_cols, int box_rows);
 // Device word shared by all kernels with bounded waits (allocated on first use, one per device).
 int32_t* device_status_word();
 

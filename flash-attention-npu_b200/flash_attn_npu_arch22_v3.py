@@ -11,9 +11,9 @@ import weakref
 
 import torch
 
+from flash_b200 import kv8
 from flash_b200 import lib as L
 from flash_b200 import ops
-
 
 
 def _reject(cond, msg):
@@ -38,11 +38,22 @@ def fwd(q, k, v, k_new_, v_new_, q_v_, out_, cu_seqlens_q_, cu_seqlens_k_, cu_se
     _reject(seqused_q_ is not None, "NPU FlashAttention does not support seqused_q")
     _reject(cu_seqlens_k_new_ is not None, "NPU FlashAttention does not support cu_seqlens_k_new")
     _reject(seqlens_rotary_ is not None, "NPU FlashAttention does not support seqlens_rotary")
-    _reject(q_descale_ is not None or k_descale_ is not None or v_descale_ is not None,
-            "NPU FlashAttention does not support descale")
     _reject(attention_chunk != 0, "NPU FlashAttention does not support attention_chunk")
     if softmax_scale_ is None:
         softmax_scale_ = q.shape[-1] ** (-0.5)
+    if kv8.holds_codes(k, v):  # a KV cache in 8 bits: the descale arguments are its scales
+        _reject(q_descale_ is not None, "the queries of an 8-bit KV cache are fp16 or bf16: q_descale is not supported")
+        _reject(cu_seqlens_k_ is not None, "an 8-bit KV cache is contiguous or paged: cu_seqlens_k is not supported")
+        _reject(scheduler_metadata_ is not None, "scheduler_metadata is not supported with an 8-bit KV cache")
+        _reject(out_ is not None, "a pre-allocated output is not supported with an 8-bit KV cache")
+        out, lse = kv8.attention_forward_kv8(
+            q, k, v, k_descale_, v_descale_, k_new=k_new_, v_new=v_new_, cu_seqlens_q=cu_seqlens_q_, max_seqlen_q=max_seqlen_q_,
+            seqused_k=seqused_k_, cache_batch_idx=kv_batch_idx_, block_table=page_table_, rotary_cos=rotary_cos_,
+            rotary_sin=rotary_sin_, rotary_interleaved=is_rotary_interleaved, softmax_scale=softmax_scale_, causal=is_causal,
+            window_left=window_size_left, window_right=window_size_right, softcap=softcap, num_splits=num_splits)
+        return [out, lse, None, None]
+    _reject(q_descale_ is not None or k_descale_ is not None or v_descale_ is not None,
+            "NPU FlashAttention does not support descale")
     plan_bytes = _plan_bytes(scheduler_metadata_) if scheduler_metadata_ is not None else None
     if k.dim() == 3 and cu_seqlens_k_ is None and seqused_k_ is not None and page_table_ is None:
         # Packed (total_k, h_k, d) keys described by their per-sequence lengths alone: the reference's kernel takes

@@ -2,10 +2,12 @@
 
 Names and argument lists follow the reference's registrations (flash_attn_npu_v3/interface_arch22.py:63-154 forward
 with its fake :157-259, :262-360 backward; ``device_types="npu"`` there), so graphs captured against the reference
-keep their node names; the bodies call this library's extension module.  One operator is added:
+keep their node names; the bodies call this library's extension module.  Added operators:
 ``_flash_attn_forward_inplace`` is the forward for calls that bring new tokens (``k_new`` / ``v_new``), which are
 written into the KV cache: it declares that it mutates ``k`` and ``v``, which a tracing compiler has to know (the
-reference registers its forward as mutating nothing although its documented semantics append in place).
+reference registers its forward as mutating nothing although its documented semantics append in place);
+``_flash_attn_forward_kv8_inplace`` is the same for a cache held in 8 bits, whose scales change too;
+``_quantized_kvcache_append`` and ``_paged_kvcache_plan`` are the two operators around such a cache.
 """
 from __future__ import annotations
 
@@ -14,6 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 import flash_attn_npu_arch22_v3 as _ext
+from flash_b200 import kv8
 
 NS = "flash_attn_npu_arch22_v3"
 
@@ -112,6 +115,56 @@ def _(q, k, v, k_new, v_new, cu_seqlens_q=None, seqused_k=None, max_seqlen_q=Non
       rotary_cos=None, rotary_sin=None, softmax_scale=None, causal=False, window_size_left=-1, window_size_right=-1,
       softcap=0.0, rotary_interleaved=True, scheduler_metadata=None, num_splits=1, pack_gqa=None, sm_margin=0):
     return _shapes(q, v, None, cu_seqlens_q, max_seqlen_q)
+
+
+@torch.library.custom_op(f"{NS}::_flash_attn_forward_kv8_inplace", mutates_args=("k", "v", "k_descale", "v_descale"), device_types="cuda")
+def _flash_attn_forward_kv8_inplace(
+        q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_descale: torch.Tensor,
+        v_descale: torch.Tensor, cu_seqlens_q: Optional[torch.Tensor] = None, seqused_k: Optional[torch.Tensor] = None,
+        max_seqlen_q: Optional[int] = None, page_table: Optional[torch.Tensor] = None,
+        kv_batch_idx: Optional[torch.Tensor] = None, rotary_cos: Optional[torch.Tensor] = None,
+        rotary_sin: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None, causal: bool = False,
+        window_size_left: int = -1, window_size_right: int = -1, softcap: float = 0.0, rotary_interleaved: bool = True,
+        num_splits: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    return kv8.attention_forward_kv8(
+        q, k, v, k_descale, v_descale, k_new=k_new, v_new=v_new, cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q,
+        seqused_k=seqused_k, cache_batch_idx=kv_batch_idx, block_table=page_table, rotary_cos=rotary_cos, rotary_sin=rotary_sin,
+        rotary_interleaved=rotary_interleaved, softmax_scale=softmax_scale, causal=causal, window_left=window_size_left,
+        window_right=window_size_right, softcap=softcap, num_splits=num_splits)
+
+
+@_flash_attn_forward_kv8_inplace.register_fake
+def _(q, k, v, k_new, v_new, k_descale, v_descale, cu_seqlens_q=None, seqused_k=None, max_seqlen_q=None, page_table=None,
+      kv_batch_idx=None, rotary_cos=None, rotary_sin=None, softmax_scale=None, causal=False, window_size_left=-1,
+      window_size_right=-1, softcap=0.0, rotary_interleaved=True, num_splits=0):
+    return _shapes(q, v, None, cu_seqlens_q, max_seqlen_q)[:2]
+
+
+@torch.library.custom_op(f"{NS}::_quantized_kvcache_append", mutates_args=("k_cache", "v_cache", "k_descale", "v_descale"),
+                         device_types="cuda")
+def _quantized_kvcache_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                              k_descale: torch.Tensor, v_descale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    kv8.append_kv8(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping)
+
+
+@_quantized_kvcache_append.register_fake
+def _(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping):
+    return None
+
+
+@torch.library.custom_op(f"{NS}::_paged_kvcache_plan", mutates_args=("page_table",), device_types="cuda")
+def _paged_kvcache_plan(cache_seqlens: torch.Tensor, new_seqlens: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor,
+                        page_size: int, total_new: int, num_free: Optional[torch.Tensor] = None
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return kv8.kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free)
+
+
+@_paged_kvcache_plan.register_fake
+def _(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free=None):
+    b = cache_seqlens.numel()
+    new = lambda n, dtype: torch.empty((n,), dtype=dtype, device=page_table.device)  # noqa: E731
+    return (new(total_new, torch.int64), new(b + 1, torch.int32), new(b, torch.int32), new(total_new, torch.int32),
+            new(1, torch.int32))
 
 
 @torch.library.custom_op(f"{NS}::_flash_attn_backward", mutates_args=("dq", "dk", "dv"), device_types="cuda")

@@ -3,9 +3,11 @@
 Same names, argument order, defaults and return conventions as
 flash_attn_npu_v3/interface_arch22.py of the reference (:797-1138); every call funnels into the
 single positional ``flash_attn_npu_arch22_v3.fwd`` exactly like the reference (:63-154).
-Arguments the backend does not implement (qv, *_descale, attention_chunk, seqused_q,
+Arguments the backend does not implement (qv, attention_chunk, seqused_q,
 cu_seqlens_k_new, rotary_seqlens, cache_leftpad) must keep their defaults, as in the reference
-(csrc/arch22/flash_attn_npu_v3/flash_api.cpp:150-162).  ``flash_attn_func`` and
+(csrc/arch22/flash_attn_npu_v3/flash_api.cpp:150-162); so must *_descale, but for k_descale and v_descale of
+``flash_attn_with_kvcache`` over a cache held in 8 bits.  ``paged_kvcache_plan`` and ``quantized_kvcache_append`` are the two
+operators around such a cache; the reference has neither.  ``flash_attn_func`` and
 ``flash_attn_varlen_func`` are differentiable (backward through ``flash_attn_npu_arch22_v3.bwd``).
 
 Eager calls with ordinary arguments take the native host path (csrc/torch_binding.cpp), which answers NotImplemented for
@@ -18,7 +20,7 @@ from typing import Optional, Union
 import torch
 
 import flash_attn_npu_arch22_v3 as _ext
-from flash_b200 import _native
+from flash_b200 import _native, kv8
 
 from . import custom_ops as _ops  # registers the torch.library operators the calls below go through
 
@@ -169,9 +171,23 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
                             sm_margin=0, return_softmax_lse=False):
     """KV-cache attention; q is (b, s_q, h, d) or (total_q, h, d) with cu_seqlens_q + max_seqlen_q.
     Returns out, or (out, softmax_lse, out_accum, softmax_lse_accum) when return_softmax_lse
-    (the last two are empty tensors, as in the reference :1095)."""
+    (the last two are empty tensors, as in the reference :1095).
+
+    k_cache / v_cache may hold 8-bit codes (torch.float8_e4m3fn or torch.int8) with k_descale / v_descale fp32 of shape
+    (pages or cache rows, blocks of tokens, nheads_k): an element stands for code * scale of its (block, head).  Blocks have
+    equal, whole multiples of 16 tokens: a page (or a cache row) divided by the second dimension.  Head dims are multiples of 16.  k / v are then
+    appended as ``quantized_kvcache_append`` does -- codes and scales change in place -- and attended to as the cache
+    holds them.  scheduler_metadata and q_descale are refused."""
     if softmax_scale is None:
         softmax_scale = _default_scale(q, qv)
+    if kv8.holds_codes(k_cache, v_cache):
+        out, lse = _kvcache_8bit(
+            q, k_cache, v_cache, k, v, qv, rotary_cos, rotary_sin, cache_seqlens, cache_batch_idx, cache_leftpad, page_table,
+            cu_seqlens_q, cu_seqlens_k_new, max_seqlen_q, rotary_seqlens, q_descale, k_descale, v_descale, softmax_scale, causal,
+            window_size, attention_chunk, softcap, rotary_interleaved, scheduler_metadata, num_splits, pack_gqa, sm_margin)
+        if not return_softmax_lse:
+            return out
+        return out, lse, torch.empty((0,), device=q.device), torch.empty((0,), device=q.device)
     if (qv is None and cache_leftpad is None and cu_seqlens_k_new is None and rotary_seqlens is None and q_descale is None
             and k_descale is None and v_descale is None and attention_chunk == 0 and not isinstance(cache_seqlens, int)
             and not torch.compiler.is_compiling()
@@ -197,6 +213,88 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
                                rotary_interleaved=rotary_interleaved, scheduler_metadata=scheduler_metadata,
                                num_splits=num_splits, pack_gqa=pack_gqa, sm_margin=sm_margin)
     return (out, lse, *rest) if return_softmax_lse else out
+
+
+def _operators_only(*tensors):
+    """Whether a call has to go through the registered operators: it is traced, under a mode, or asks for a gradient."""
+    return (torch.compiler.is_compiling() or not _native.plain_eager() or
+            any(t is not None and (type(t) not in (torch.Tensor, torch.nn.Parameter) or (t.requires_grad and torch.is_grad_enabled()))
+                for t in tensors))
+
+
+def _wrote(*tensors):
+    """The tensors were written to in place."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
+def _kvcache_8bit(q, k_cache, v_cache, k, v, qv, rotary_cos, rotary_sin, cache_seqlens, cache_batch_idx, cache_leftpad, page_table,
+                  cu_seqlens_q, cu_seqlens_k_new, max_seqlen_q, rotary_seqlens, q_descale, k_descale, v_descale, softmax_scale,
+                  causal, window_size, attention_chunk, softcap, rotary_interleaved, scheduler_metadata, num_splits, pack_gqa, sm_margin):
+    if isinstance(cache_seqlens, int):
+        b = q.shape[0] if cu_seqlens_q is None else cu_seqlens_q.shape[0] - 1
+        cache_seqlens = torch.full((b,), cache_seqlens, dtype=torch.int32, device=k_cache.device)
+    q, k, v = [maybe_contiguous(x) for x in (q, k, v)]
+    cu_seqlens_q, cache_seqlens, page_table, cache_batch_idx = [
+        maybe_contiguous(x) for x in (cu_seqlens_q, cache_seqlens, page_table, cache_batch_idx)]
+    refused = (qv, cu_seqlens_k_new, cache_leftpad, rotary_seqlens, q_descale, scheduler_metadata)
+    through = _operators_only(q, k_cache, v_cache, k, v, k_descale, v_descale, rotary_cos, rotary_sin)
+    if k is not None and through and not any(x is not None for x in refused) and attention_chunk == 0:
+        return _ops._flash_attn_forward_kv8_inplace(
+            q, k_cache, v_cache, k, v, k_descale, v_descale, cu_seqlens_q, cache_seqlens, max_seqlen_q, page_table, cache_batch_idx,
+            rotary_cos, rotary_sin, softmax_scale, causal, window_size[0], window_size[1], softcap, rotary_interleaved, num_splits)
+    args = (q, k_cache, v_cache, k, v, qv, None, cu_seqlens_q, None, cu_seqlens_k_new, None, cache_seqlens, max_seqlen_q, None,
+            page_table, cache_batch_idx, cache_leftpad, rotary_cos, rotary_sin, rotary_seqlens, q_descale, k_descale, v_descale,
+            softmax_scale, causal, window_size[0], window_size[1], attention_chunk, softcap, rotary_interleaved, scheduler_metadata,
+            num_splits, pack_gqa, sm_margin)
+    if through and k is None and v is None:
+        return _ops._flash_attn_forward(*args)[:2]
+    out, lse = _ext.fwd(*args)[:2]
+    if k is not None:
+        _wrote(k_cache, v_cache, k_descale, v_descale)
+    return out, lse
+
+
+def quantized_kvcache_append(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping) -> None:
+    """Writes new tokens k, v (total, nheads_k, headdim) into an 8-bit KV cache, in place: codes into k_cache / v_cache
+    (pages or rows, tokens, nheads_k, headdim; torch.float8_e4m3fn or torch.int8), one fp32 scale for each (block of tokens,
+    head) into k_descale / v_descale (pages or rows, blocks, nheads_k).
+
+    slot_mapping (total,) int64: page * tokens of a page + row of each token, negative for rows of padding (skipped).  The new
+    tokens of one block must be neighbours in the batch with consecutive slots, as ``paged_kvcache_plan`` gives them, and a
+    page that is written to must belong to one sequence.
+
+    A scale is the smallest power of two, 2^-40 at least, that brings the block's largest finite element into the codes' range
+    (448 for e4m3, 127 for int8).  Where tokens are there in front of the new ones, the block keeps its scale if that is larger, and
+    otherwise their codes are expressed in the new one; a block whose first token is written starts afresh.  Codes are rounded
+    to nearest even; infinities saturate; NaN is stored as NaN (e4m3) or 0 (int8)."""
+    k, v = maybe_contiguous(k), maybe_contiguous(v)
+    if _operators_only(k, v, k_cache, v_cache, k_descale, v_descale):
+        return _ops._quantized_kvcache_append(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping)
+    kv8.append_kv8(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping)
+    _wrote(k_cache, v_cache, k_descale, v_descale)
+
+
+def paged_kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size: int, total_new: int,
+                       num_free: Optional[torch.Tensor] = None):
+    """One serving step's bookkeeping for a paged KV cache, on the GPU and without a look at the lengths on the host.
+
+    Request r holds cache_seqlens[r] tokens and brings new_seqlens[r] (int32, (batch,)).  The pages it lacks are taken off
+    free_pages (int32; its first num_free[0] entries where num_free, an int32 tensor of one element, is given) in request
+    order and written into its row of page_table (batch, max_pages) int32, in place.  A request that its row or the free list
+    has no room for is left as it was.  total_new: rows of the packed batch, the sum of new_seqlens or more (the rows behind
+    are padding).  Up to 16384 requests.
+
+    Returns (slot_mapping (total_new,) int64: where ``quantized_kvcache_append`` puts each packed token, -1 for padding and
+    requests left out; cu_seqlens (batch + 1,) int32 offsets of the requests in the packed batch; cache_seqlens afterwards
+    (batch,) int32; positions (total_new,) int32 of the tokens in their sequences, 0 for padding; pages taken (1,) int32: the
+    free list's first ones)."""
+    if _operators_only(cache_seqlens, new_seqlens, page_table, free_pages, num_free):
+        return _ops._paged_kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free)
+    got = kv8.kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free)
+    _wrote(page_table)
+    return got
 
 
 def get_scheduler_metadata(batch_size, max_seqlen_q, max_seqlen_k, num_heads_q, num_heads_kv, headdim,

@@ -88,6 +88,42 @@ class Exchange(C.Structure):
                 ("timeout_cycles", _i64)]
 
 
+CODE_E4M3, CODE_INT8 = 0, 1
+
+
+class Kv8Cache(C.Structure):
+    """Mirror of ``fa_kv8_cache``."""
+    _fields_ = (
+        [("k_scale", _p), ("v_scale", _p)]
+        + [(f"{t}_{s}_stride", _i64) for t in ("ks", "vs") for s in ("outer", "block", "head")]
+        + [("scale_block", _i32), ("code", _i32)]
+    )
+
+
+class Kv8AppendParams(C.Structure):
+    """Mirror of ``fa_kv8_append_params``."""
+    _fields_ = (
+        [(n, _p) for n in ("k", "v", "k_cache", "v_cache", "slots")]
+        + [(n, _i64) for n in (
+            "k_tok_stride", "k_head_stride", "v_tok_stride", "v_head_stride",
+            "kc_outer_stride", "kc_row_stride", "kc_head_stride",
+            "vc_outer_stride", "vc_row_stride", "vc_head_stride", "total")]
+        + [(n, _i32) for n in ("kv_outer", "rows", "h_k", "d", "dtype", "num_sm")]
+        + [("c", Kv8Cache)]
+    )
+
+
+class KvcachePlanParams(C.Structure):
+    """Mirror of ``fa_kvcache_plan_params``."""
+    _fields_ = (
+        [(n, _p) for n in ("have", "add", "table", "free_pages", "num_free", "slots", "cu_new", "after", "positions", "pages_taken")]
+        + [("table_stride", _i64), ("total", _i64)]
+        + [(n, _i32) for n in ("b", "cols", "page_size", "n_free", "num_sm")]
+    )
+
+
+PLAN_MAX_REQUESTS = 16384  # FA_B200_PLAN_MAX_REQUESTS
+
 # every symbol include/fa_b200.h declares
 EXPORTS = (
     "fa_b200_fwd", "fa_b200_fwd_alloc", "fa_b200_fwd_noalloc", "fa_b200_fwd_plan", "fa_b200_combine", "fa_b200_normalize_window",
@@ -96,6 +132,7 @@ EXPORTS = (
     "fa_b200_plan_encode", "fa_b200_plan_decode", "fa_b200_fwd_planned",
     "fa_b200_exchange_bytes", "fa_b200_exchange_alloc", "fa_b200_exchange_open", "fa_b200_exchange_close",
     "fa_b200_exchange_free", "fa_b200_fwd_exchange_workspace", "fa_b200_fwd_exchange",
+    "fa_b200_kv8_fwd", "fa_b200_kv8_fwd_workspace", "fa_b200_kv8_fwd_alloc", "fa_b200_kv8_append", "fa_b200_kvcache_plan",
 )
 PLAN_BYTES = 192  # FA_B200_PLAN_BYTES
 
@@ -141,6 +178,14 @@ def load() -> C.CDLL:
     lib.fa_b200_bwd.restype = C.c_int
     lib.fa_b200_bwd_workspace_bytes.argtypes = [C.POINTER(BwdParams)]
     lib.fa_b200_bwd_workspace_bytes.restype = C.c_size_t
+    lib.fa_b200_kv8_fwd.argtypes = [C.POINTER(FwdParams), C.POINTER(Kv8Cache), _p, C.c_size_t, _p]
+    lib.fa_b200_kv8_fwd.restype = C.c_int
+    lib.fa_b200_kv8_fwd_workspace.argtypes = [C.POINTER(FwdParams), C.POINTER(Kv8Cache)]
+    lib.fa_b200_kv8_fwd_workspace.restype = C.c_size_t
+    lib.fa_b200_kv8_append.argtypes = [C.POINTER(Kv8AppendParams), _p]
+    lib.fa_b200_kv8_append.restype = C.c_int
+    lib.fa_b200_kvcache_plan.argtypes = [C.POINTER(KvcachePlanParams), _p]
+    lib.fa_b200_kvcache_plan.restype = C.c_int
     lib.fa_b200_combine.argtypes = [C.POINTER(CombineParams), _p]
     lib.fa_b200_combine.restype = C.c_int
     lib.fa_b200_normalize_window.argtypes = [_i32, _i32, _i32] + [C.POINTER(_i32)] * 4

@@ -31,6 +31,8 @@
  *   fa_b200_normalize_window    the window normalisation block, flash_api.cpp:483-494
  *   fa_b200_check_status        (none: device-side wait watchdog of this library)
  *   fa_b200_fwd_noalloc         (none: allocation-free variant of fa_b200_fwd)
+ *   fa_b200_kv8_* /             (none: serving from a KV cache held in 8 bits; the reference's forward refuses the
+ *   fa_b200_kvcache_plan        k_descale / v_descale arguments, csrc/arch22/flash_attn_npu_v3/flash_api.cpp:150-162)
  */
 #ifndef FA_B200_H
 #define FA_B200_H
@@ -273,6 +275,80 @@ int fa_b200_exchange_close(void* ptr);
 int fa_b200_exchange_free(void* ptr);
 size_t fa_b200_fwd_exchange_workspace(const fa_fwd_params* p);
 int fa_b200_fwd_exchange(const fa_fwd_params* p, void* workspace, size_t workspace_bytes, const fa_exchange* x, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * KV caches held in 8 bits.  k / v of the cache hold codes, one byte per element, and a scale belongs to every (block of
+ * scale_block tokens, kv head) of K and of V: an element stands for code * scale.  scale_block is a multiple of 16 that
+ * divides the rows of a page (paged) or of a cache row (contiguous).  Head dims up to 256, multiples of 16; strides of the
+ * codes are multiples of 16.
+ * ------------------------------------------------------------------------------------------------ */
+enum fa_code { FA_CODE_E4M3 = 0, FA_CODE_INT8 = 1 };
+typedef struct fa_kv8_cache {
+  float* k_scale; /* [outer: page or cache row][block of tokens in it][kv head], any strides (elements) */
+  float* v_scale;
+  int64_t ks_outer_stride, ks_block_stride, ks_head_stride;
+  int64_t vs_outer_stride, vs_block_stride, vs_head_stride;
+  int32_t scale_block;
+  int32_t code; /* enum fa_code, of K and V alike */
+} fa_kv8_cache;
+
+/* fa_b200_fwd over such a cache: p->k / p->v are codes (strides in elements), p->dtype is the type of q, o, k_new and v_new.
+ * Dense or packed (cu_seqlens_q) queries; contiguous (cache_batch_idx) or paged caches; causal, window, softcap, rotary
+ * with k_new.  New tokens are appended as fa_b200_kv8_append does and then attended to as the cache holds them.
+ * Not here: cu_seqlens_k, alibi, sharded positions, partial_out.  num_splits as in fa_b200_fwd; p->kernel is not read. */
+int fa_b200_kv8_fwd(const fa_fwd_params* p, const fa_kv8_cache* c, void* workspace, size_t workspace_bytes, void* stream);
+size_t fa_b200_kv8_fwd_workspace(const fa_fwd_params* p, const fa_kv8_cache* c); /* 0 also for a call that would be refused */
+/* ... with the workspace taken from a callback, as in fa_b200_fwd_alloc. */
+int fa_b200_kv8_fwd_alloc(const fa_fwd_params* p, const fa_kv8_cache* c, void* (*alloc)(size_t bytes, void* ctx), void* ctx,
+                          void* stream);
+
+/* New tokens -> codes and scales.  Token t goes to row slots[t] % rows of page slots[t] / rows; a slot that is negative (padding) or outside
+ * the cache (reported by fa_b200_check_status) is skipped.  The new tokens of one scale block must be neighbours in the batch
+ * with consecutive slots, as fa_b200_kvcache_plan gives them, and no other call may write the block meanwhile.  The scale is the
+ * smallest power of two, 2^-40 at least, that brings the largest finite element into the codes' range (e4m3: 448, int8: 127).
+ * A block whose first rows are not among the new ones keeps its scale if that is larger, else its earlier rows are
+ * expressed in the new one; a block whose first row is written starts afresh.  Rows behind the new ones are not touched.  Codes are rounded to
+ * nearest even; infinities saturate; NaN is stored as NaN (e4m3) or 0 (int8). */
+typedef struct fa_kv8_append_params {
+  const void* k; /* (total, h_k, d), fp16 or bf16 */
+  const void* v;
+  void* k_cache; /* (kv_outer, rows, h_k, d) codes */
+  void* v_cache;
+  const int64_t* slots; /* (total) */
+  int64_t k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  int64_t kc_outer_stride, kc_row_stride, kc_head_stride;
+  int64_t vc_outer_stride, vc_row_stride, vc_head_stride;
+  int64_t total;
+  int32_t kv_outer, rows, h_k, d;
+  int32_t dtype;  /* enum fa_dtype of k, v */
+  int32_t num_sm; /* 0 = query the current device */
+  fa_kv8_cache c;
+} fa_kv8_append_params;
+int fa_b200_kv8_append(const fa_kv8_append_params* p, void* stream);
+
+/* One serving step's bookkeeping from the requests' lengths, on the device.  Request r holds have[r] tokens in ceil(have / page_size)
+ * pages named by its row of the table and brings add[r] more; the pages it lacks are taken off free_pages in request order and written into
+ * its row.  A request that its row or the free list has no room for stays as it was.  Outputs: cu_new (b + 1) offsets of the
+ * requests' new tokens in the packed batch; after (b) lengths afterwards; slots (total): page * page_size + row of each packed
+ * token, -1 for tokens of a refused request and rows behind the last one; positions (total) in their sequence, 0 behind the last;
+ * pages_taken (1).  Negative lengths are refused like that and reported by fa_b200_check_status. */
+#define FA_B200_PLAN_MAX_REQUESTS 16384
+typedef struct fa_kvcache_plan_params {
+  const int32_t* have;
+  const int32_t* add;
+  int32_t* table; /* (b, cols), row stride table_stride */
+  const int32_t* free_pages;
+  const int32_t* num_free; /* entries of free_pages that count, on the device; NULL: all n_free */
+  int64_t* slots;
+  int32_t* cu_new;
+  int32_t* after;
+  int32_t* positions;
+  int32_t* pages_taken;
+  int64_t table_stride, total;
+  int32_t b, cols, page_size, n_free;
+  int32_t num_sm; /* 0 = query the current device */
+} fa_kvcache_plan_params;
+int fa_b200_kvcache_plan(const fa_kvcache_plan_params* p, void* stream);
 
 /* Merge of split partials (also used across GPUs). */
 int fa_b200_combine(const fa_combine_params* p, void* stream);

@@ -74,6 +74,10 @@ bool plain(const Tensor& t) {
 bool data_tensor(const Tensor* t, const Tensor& q, int64_t dim) {  // a 16-bit operand beside q
   return t && plain(*t) && t->scalar_type() == q.scalar_type() && t->device() == q.device() && t->dim() == dim && t->stride(-1) == 1;
 }
+bool code_tensor(const Tensor* t, const Tensor& q) {  // a KV cache in 8 bits
+  return t && plain(*t) && (t->scalar_type() == at::kFloat8_e4m3fn || t->scalar_type() == at::kChar) && t->device() == q.device() &&
+         t->dim() == 4 && t->stride(-1) == 1;
+}
 bool index_tensor(const Tensor* t, const Tensor& q, int64_t numel) {  // optional contiguous int32 vector
   return !t || (plain(*t) && t->scalar_type() == at::kInt && t->device() == q.device() && t->dim() == 1 && t->numel() == numel &&
                 t->is_contiguous());
@@ -84,6 +88,7 @@ const void* ptr(const Tensor* t) { return t ? t->const_data_ptr() : nullptr; }
 struct FwdArgs {
   const Tensor *q, *k, *v, *k_new = nullptr, *v_new = nullptr, *cu_q = nullptr, *cu_k = nullptr, *seqused_k = nullptr,
                *batch_idx = nullptr, *table = nullptr, *cos = nullptr, *sin = nullptr, *alibi = nullptr;
+  const fa_kv8_cache* kv8 = nullptr;  // k, v are codes with these scales
   int64_t max_q = 0, max_k = 0, wl = -1, wr = -1, num_splits = 0;
   bool causal = false, interleaved = true;
   double scale = 1.0, softcap = 0.0;
@@ -98,7 +103,10 @@ bool fill_params(const FwdArgs& a, fa_fwd_params& p) {
   const Tensor &q = *a.q;
   const bool packed_q = a.cu_q != nullptr, packed_k = a.cu_k != nullptr;
   if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) return false;
-  if (q.dim() != (packed_q ? 3 : 4) || !data_tensor(a.k, q, packed_k ? 3 : 4) || !data_tensor(a.v, q, packed_k ? 3 : 4)) return false;
+  if (q.dim() != (packed_q ? 3 : 4)) return false;
+  if (a.kv8 ? !code_tensor(a.k, q) || !code_tensor(a.v, q) || a.k->scalar_type() != a.v->scalar_type()
+            : !data_tensor(a.k, q, packed_k ? 3 : 4) || !data_tensor(a.v, q, packed_k ? 3 : 4))
+    return false;
   const Tensor &k = *a.k, &v = *a.v;
   if (k.sizes() != v.sizes() || k.size(-1) != q.size(-1)) return false;
   const int64_t d = q.size(-1), h = q.size(-2), h_k = k.size(-2);
@@ -221,7 +229,8 @@ bool launch_forward(const FwdArgs& a, fa_fwd_params& p, Tensor& out, Tensor& lse
   Scratch ws{q.device(), Tensor(), nullptr};
   void* stream = at::cuda::getCurrentCUDAStream(q.device().index()).stream();
   NoGil nogil;
-  const int rc = fa_b200_fwd_alloc(&p, a.plan, (size_t)a.plan_bytes, alloc_workspace, &ws, stream);
+  const int rc = a.kv8 ? fa_b200_kv8_fwd_alloc(&p, a.kv8, alloc_workspace, &ws, stream)
+                       : fa_b200_fwd_alloc(&p, a.plan, (size_t)a.plan_bytes, alloc_workspace, &ws, stream);
   if (ws.error) std::rethrow_exception(ws.error);
   return rc == FA_OK;
 }
@@ -372,12 +381,159 @@ PyObject* kvcache(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ KV caches in 8 bits
+// The scales of a cache of codes; false: not an ordinary one.
+bool fill_scales(const Tensor* k, const Tensor* v, const Tensor* ks, const Tensor* vs, fa_kv8_cache& c) {
+  std::memset(&c, 0, sizeof(c));
+  if (!k || !v || !code_tensor(k, *k) || !code_tensor(v, *k) || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type()) return false;
+  for (const Tensor* t : {ks, vs})
+    if (!t || !plain(*t) || t->scalar_type() != at::kFloat || t->device() != k->device() || t->dim() != 3 || t->size(0) != k->size(0) ||
+        t->size(1) != ks->size(1) || t->size(1) <= 0 || t->size(2) != k->size(2) || k->size(1) % t->size(1) != 0)
+      return false;
+  c.k_scale = const_cast<float*>((const float*)ptr(ks));
+  c.v_scale = const_cast<float*>((const float*)ptr(vs));
+  c.ks_outer_stride = ks->stride(0); c.ks_block_stride = ks->stride(1); c.ks_head_stride = ks->stride(2);
+  c.vs_outer_stride = vs->stride(0); c.vs_block_stride = vs->stride(1); c.vs_head_stride = vs->stride(2);
+  c.scale_block = (int32_t)(k->size(1) / ks->size(1));
+  c.code = k->scalar_type() == at::kChar ? FA_CODE_INT8 : FA_CODE_E4M3;
+  return true;
+}
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+bool may_write(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->is_inference()) return false;
+  return true;
+}
+void wrote(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) torch::autograd::impl::bump_version(*t);
+}
+PyObject* tuple_of(std::initializer_list<Tensor> ts) {
+  PyObject* t = PyTuple_New((Py_ssize_t)ts.size());
+  if (!t) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor& x : ts) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(x));
+  return t;
+}
+
+// kvcache8(q, k_cache, v_cache, k, v, cu_seqlens_q, max_seqlen_q, cache_seqlens, cache_batch_idx, page_table, rotary_cos, rotary_sin,
+//          rotary_interleaved, k_descale, v_descale, softmax_scale, causal, window_left, window_right, softcap, num_splits)
+//   -> (out, lse), or NotImplemented
+PyObject* kvcache8(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  FwdArgs a;
+  fa_fwd_params p;
+  fa_kv8_cache c;
+  const Tensor *ks, *vs;
+  if (n != 21 || !plain_eager()) return not_implemented();
+  if (!as_tensor(o[0], a.q) || !as_tensor(o[1], a.k) || !as_tensor(o[2], a.v) || !as_tensor(o[3], a.k_new) || !as_tensor(o[4], a.v_new) ||
+      !as_tensor(o[5], a.cu_q) || (a.cu_q && !as_int(o[6], a.max_q)) || !as_tensor(o[7], a.seqused_k) || !as_tensor(o[8], a.batch_idx) ||
+      !as_tensor(o[9], a.table) || !as_tensor(o[10], a.cos) || !as_tensor(o[11], a.sin) || !as_bool(o[12], a.interleaved) ||
+      !as_tensor(o[13], ks) || !as_tensor(o[14], vs) || !as_float(o[15], a.scale) || !as_bool(o[16], a.causal) || !as_int(o[17], a.wl) ||
+      !as_int(o[18], a.wr) || !as_float(o[19], a.softcap) || !as_int(o[20], a.num_splits))
+    return not_implemented();
+  if (!a.q || !fill_scales(a.k, a.v, ks, vs, c) || a.k->device() != a.q->device()) return not_implemented();
+  a.kv8 = &c;
+  if (wants_grad({a.q, a.k, a.v, a.k_new, a.v_new, a.cos, a.sin, ks, vs}) || !fill_params(a, p)) return not_implemented();
+  if (a.k_new && !may_write({a.k, a.v, ks, vs})) return not_implemented();
+  Tensor out, lse;
+  if (!launch_forward(a, p, out, lse)) return not_implemented();
+  if (a.k_new) wrote({a.k, a.v, ks, vs});
+  return two(std::move(out), std::move(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// append8(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping) -> None, or NotImplemented
+PyObject* append8(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *k, *v, *kc, *vc, *ks, *vs, *slots;
+  fa_kv8_append_params p;
+  std::memset(&p, 0, sizeof(p));
+  if (n != 7 || !plain_eager()) return not_implemented();
+  if (!as_tensor(o[0], k) || !as_tensor(o[1], v) || !as_tensor(o[2], kc) || !as_tensor(o[3], vc) || !as_tensor(o[4], ks) ||
+      !as_tensor(o[5], vs) || !as_tensor(o[6], slots) || !k || !plain(*k) || k->dim() != 3 || k->stride(-1) != 1 || !data_tensor(v, *k, 3) ||
+      v->sizes() != k->sizes() || (k->scalar_type() != at::kHalf && k->scalar_type() != at::kBFloat16) || !fill_scales(kc, vc, ks, vs, p.c) ||
+      kc->device() != k->device() || kc->size(2) != k->size(1) || kc->size(3) != k->size(2) || !slots || !plain(*slots) ||
+      slots->scalar_type() != at::kLong || slots->device() != k->device() || slots->dim() != 1 || slots->numel() != k->size(0) ||
+      !slots->is_contiguous() || wants_grad({k, v, kc, vc, ks, vs}) || !may_write({kc, vc, ks, vs}))
+    return not_implemented();
+  p.k = ptr(k); p.v = ptr(v); p.slots = (const int64_t*)ptr(slots);
+  p.k_cache = const_cast<void*>(ptr(kc)); p.v_cache = const_cast<void*>(ptr(vc));
+  p.k_tok_stride = k->stride(0); p.k_head_stride = k->stride(1);
+  p.v_tok_stride = v->stride(0); p.v_head_stride = v->stride(1);
+  p.kc_outer_stride = kc->stride(0); p.kc_row_stride = kc->stride(1); p.kc_head_stride = kc->stride(2);
+  p.vc_outer_stride = vc->stride(0); p.vc_row_stride = vc->stride(1); p.vc_head_stride = vc->stride(2);
+  p.total = k->size(0); p.h_k = (int32_t)k->size(1); p.d = (int32_t)k->size(2);
+  p.kv_outer = (int32_t)kc->size(0); p.rows = (int32_t)kc->size(1);
+  p.dtype = k->scalar_type() == at::kBFloat16 ? FA_BF16 : FA_FP16;
+  p.num_sm = at::cuda::getDeviceProperties(k->device().index())->multiProcessorCount;
+  c10::cuda::CUDAGuard guard(k->device());
+  int rc;
+  {
+    void* stream = at::cuda::getCurrentCUDAStream(k->device().index()).stream();
+    NoGil nogil;
+    rc = fa_b200_kv8_append(&p, stream);
+  }
+  if (rc != FA_OK) return not_implemented();
+  wrote({kc, vc, ks, vs});
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// step_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free)
+//   -> (slots, cu_seqlens, cache_seqlens afterwards, positions, pages taken), or NotImplemented
+PyObject* step_plan(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *have, *add, *table, *free, *num_free;
+  int64_t page = 0, total = 0;
+  if (n != 7 || !plain_eager()) return not_implemented();
+  if (!as_tensor(o[0], have) || !as_tensor(o[1], add) || !as_tensor(o[2], table) || !as_tensor(o[3], free) || !as_int(o[4], page) ||
+      !as_int(o[5], total) || !as_tensor(o[6], num_free) || !have || !add || !table || !free || !plain(*table) ||
+      table->scalar_type() != at::kInt || table->dim() != 2 || total < 0 || page <= 0 || page > INT32_MAX)
+    return not_implemented();
+  const int64_t b = have->numel(), cols = table->size(1);
+  if (!index_tensor(have, *table, b) || !index_tensor(add, *table, b) || !index_tensor(free, *table, free->numel()) ||
+      !index_tensor(num_free, *table, 1) || table->size(0) != b || table->stride(1) != 1 || (b > 1 && table->stride(0) < cols) ||
+      !may_write({table}))
+    return not_implemented();
+  c10::cuda::CUDAGuard guard(table->device());
+  const auto i32 = at::TensorOptions().dtype(at::kInt).device(table->device());
+  const Tensor slots = at::empty({total}, i32.dtype(at::kLong)), positions = at::empty({total}, i32), cu = at::empty({b + 1}, i32),
+               after = at::empty({b}, i32), taken = at::empty({1}, i32);
+  fa_kvcache_plan_params p;
+  std::memset(&p, 0, sizeof(p));
+  p.have = (const int32_t*)ptr(have); p.add = (const int32_t*)ptr(add); p.table = const_cast<int32_t*>((const int32_t*)ptr(table));
+  p.free_pages = (const int32_t*)ptr(free); p.num_free = (const int32_t*)ptr(num_free);
+  p.slots = slots.data_ptr<int64_t>(); p.cu_new = cu.data_ptr<int32_t>(); p.after = after.data_ptr<int32_t>();
+  p.positions = positions.data_ptr<int32_t>(); p.pages_taken = taken.data_ptr<int32_t>();
+  p.table_stride = table->stride(0); p.total = total;
+  p.b = (int32_t)b; p.cols = (int32_t)cols; p.page_size = (int32_t)page; p.n_free = (int32_t)free->numel();
+  p.num_sm = at::cuda::getDeviceProperties(table->device().index())->multiProcessorCount;
+  int rc;
+  {
+    void* stream = at::cuda::getCurrentCUDAStream(table->device().index()).stream();
+    NoGil nogil;
+    rc = fa_b200_kvcache_plan(&p, stream);
+  }
+  if (rc != FA_OK) return not_implemented();
+  wrote({table});
+  return tuple_of({slots, cu, after, positions, taken});
+  END_HANDLE_TH_ERRORS
+}
+
 // plain_eager() -> bool: no mode, transform or trace is active that every function here would decline for
 PyObject* py_plain_eager(PyObject*, PyObject*) { return PyBool_FromLong(plain_eager()); }
 
 PyMethodDef methods[] = {
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "dense or packed attention; NotImplemented: use the Python path"},
     {"kvcache", (PyCFunction)(void (*)(void))kvcache, METH_FASTCALL, "attention over a KV cache; NotImplemented: use the Python path"},
+    {"kvcache8", (PyCFunction)(void (*)(void))kvcache8, METH_FASTCALL, "attention over an 8-bit KV cache; NotImplemented: use the Python path"},
+    {"append8", (PyCFunction)(void (*)(void))append8, METH_FASTCALL, "new tokens into an 8-bit KV cache; NotImplemented: use the Python path"},
+    {"step_plan", (PyCFunction)(void (*)(void))step_plan, METH_FASTCALL, "pages and slots of a serving step; NotImplemented: use the Python path"},
     {"plain_eager", py_plain_eager, METH_NOARGS, "False: a mode, transform or trace is active and every function here declines"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of the public attention calls.", -1, methods};

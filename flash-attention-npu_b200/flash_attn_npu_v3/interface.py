@@ -181,6 +181,14 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
     if softmax_scale is None:
         softmax_scale = _default_scale(q, qv)
     if kv8.holds_codes(k_cache, v_cache):
+        if (qv is None and cache_leftpad is None and cu_seqlens_k_new is None and rotary_seqlens is None and q_descale is None
+                and attention_chunk == 0 and scheduler_metadata is None and not isinstance(cache_seqlens, int)
+                and not torch.compiler.is_compiling()):
+            r = _native.kvcache8(q, k_cache, v_cache, k, v, cu_seqlens_q, max_seqlen_q, cache_seqlens, cache_batch_idx, page_table,
+                                 rotary_cos, rotary_sin, rotary_interleaved, k_descale, v_descale, softmax_scale, causal,
+                                 window_size[0], window_size[1], softcap, num_splits)
+            if r is not NotImplemented:
+                return (*r, torch.empty((0,), device=q.device), torch.empty((0,), device=q.device)) if return_softmax_lse else r[0]
         out, lse = _kvcache_8bit(
             q, k_cache, v_cache, k, v, qv, rotary_cos, rotary_sin, cache_seqlens, cache_batch_idx, cache_leftpad, page_table,
             cu_seqlens_q, cu_seqlens_k_new, max_seqlen_q, rotary_seqlens, q_descale, k_descale, v_descale, softmax_scale, causal,
@@ -269,6 +277,8 @@ def quantized_kvcache_append(k, v, k_cache, v_cache, k_descale, v_descale, slot_
     (448 for e4m3, 127 for int8).  Where tokens are there in front of the new ones, the block keeps its scale if that is larger, and
     otherwise their codes are expressed in the new one; a block whose first token is written starts afresh.  Codes are rounded
     to nearest even; infinities saturate; NaN is stored as NaN (e4m3) or 0 (int8)."""
+    if not torch.compiler.is_compiling() and _native.append8(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping) is None:
+        return
     k, v = maybe_contiguous(k), maybe_contiguous(v)
     if _operators_only(k, v, k_cache, v_cache, k_descale, v_descale):
         return _ops._quantized_kvcache_append(k, v, k_cache, v_cache, k_descale, v_descale, slot_mapping)
@@ -290,6 +300,10 @@ def paged_kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_
     requests left out; cu_seqlens (batch + 1,) int32 offsets of the requests in the packed batch; cache_seqlens afterwards
     (batch,) int32; positions (total_new,) int32 of the tokens in their sequences, 0 for padding; pages taken (1,) int32: the
     free list's first ones)."""
+    if not torch.compiler.is_compiling():
+        got = _native.step_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free)
+        if got is not NotImplemented:
+            return got
     if _operators_only(cache_seqlens, new_seqlens, page_table, free_pages, num_free):
         return _ops._paged_kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free)
     got = kv8.kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, total_new, num_free)

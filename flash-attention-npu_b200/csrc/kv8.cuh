@@ -171,7 +171,7 @@ struct Kv8Walk {
       int idx = blockIdx.x;
       const int h = idx % p.a.h_k;
       idx /= p.a.h_k;
-      const int mb = idx % p.m_blocks;
+      const int mb = p.m_blocks - 1 - idx % p.m_blocks;  // the last rows see most keys
       idx /= p.m_blocks;
       const int split = idx % p.num_splits, b = idx / p.num_splits;
       int lo, hi;

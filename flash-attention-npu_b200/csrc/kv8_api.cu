@@ -38,7 +38,7 @@ struct Kv8Plan {
   Kv8Params p;
   Kv8TileInfo tile;
   int hd, grid;
-  bool wide;
+  bool wide, tiled;
   size_t lse_bytes, workspace_bytes;
 };
 
@@ -109,7 +109,8 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   const int rows_max = a.seqlen_q * p.group;
   out->hd = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
   out->wide = rows_max > 16;
-  out->tile = kv8_decode_info(out->hd, out->wide);
+  out->tiled = rows_max > 32;
+  out->tile = out->tiled ? kv8_tile_info(out->hd) : kv8_decode_info(out->hd, out->wide);
   const Kv8TileInfo& t = out->tile;
   p.m_blocks = std::max(1, ceil_div(rows_max, t.block_m));
   p.box_rows = t.block_n;
@@ -125,12 +126,13 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   int ns = 1;
   if (a.num_splits >= 1) {
     ns = std::min(a.num_splits, max_blocks);
-  } else if (p.m_blocks == 1 && max_blocks >= 4) {
+  } else if (out->tiled) {
+    // as many key ranges as fill the chip, of at least eight blocks each
+    if (units < num_sm) ns = (int)std::max<long long>(1, std::min<long long>(num_sm / units, max_blocks / 8));
+  } else if (max_blocks >= 4) {
     p.persistent = 1;
     ns = 4;
     if (slots / units > 3) ns = (int)std::max<long long>(4, std::min<long long>(slots / units + 2, max_blocks / 2 + 1));
-  } else if (p.m_blocks > 1 && units < slots) {
-    ns = (int)std::max<long long>(1, std::min<long long>(slots / units, max_blocks / 4));
   }
   if (!p.persistent) {
     p.blocks_per_split = ceil_div(max_blocks, ns);
@@ -169,22 +171,27 @@ static int run_kv8_fwd(const fa_fwd_params& a_in, const fa_kv8_cache& c, void* w
   }
   p.status = device_status_word();
   if (!p.status) return fail(FA_ERR_CUDA, "cannot look up the device status word");
-  CUtensorMap tm_k, tm_v;
-  const int64_t rows = a.block_table ? a.page_size : a.seqlen_k, outer = a.kv_outer > 0 ? a.kv_outer : a.b;
-  const int box_cols = P.hd == 64 ? 64 : 128;
-  if (!kv8_encode_map(&tm_k, a.k, a.d, a.h_k, rows, outer, a.k_head_stride, a.k_row_stride, a.k_batch_stride, box_cols, p.box_rows) ||
-      !kv8_encode_map(&tm_v, a.v, a.d, a.h_k, rows, outer, a.v_head_stride, a.v_row_stride, a.v_batch_stride, box_cols, p.box_rows))
-    return fail(FA_ERR_CUDA, "cuTensorMapEncodeTiled failed for the KV cache");
   if (a.k_new) {
     const cudaError_t e = launch_kv8_append_dense(p, st);
     if (e != cudaSuccess) return cuda_fail("append launch", e);
     count_launches(1);
   }
-  const bool e4m3 = c.code == FA_CODE_E4M3;
-  auto* launch = P.hd == 64    ? (e4m3 ? launch_kv8_decode_64_e4m3 : launch_kv8_decode_64_int8)
-                 : P.hd == 128 ? (e4m3 ? launch_kv8_decode_128_e4m3 : launch_kv8_decode_128_int8)
-                               : (e4m3 ? launch_kv8_decode_256_e4m3 : launch_kv8_decode_256_int8);
-  const cudaError_t e = launch(P.wide, p, tm_k, tm_v, P.grid, st);
+  cudaError_t e;
+  if (P.tiled) {
+    e = P.hd == 64 ? launch_kv8_tile_64(p, P.grid, st) : P.hd == 128 ? launch_kv8_tile_128(p, P.grid, st) : launch_kv8_tile_256(p, P.grid, st);
+  } else {
+    CUtensorMap tm_k, tm_v;
+    const int64_t rows = a.block_table ? a.page_size : a.seqlen_k, outer = a.kv_outer > 0 ? a.kv_outer : a.b;
+    const int box_cols = P.hd == 64 ? 64 : 128;
+    if (!kv8_encode_map(&tm_k, a.k, a.d, a.h_k, rows, outer, a.k_head_stride, a.k_row_stride, a.k_batch_stride, box_cols, p.box_rows) ||
+        !kv8_encode_map(&tm_v, a.v, a.d, a.h_k, rows, outer, a.v_head_stride, a.v_row_stride, a.v_batch_stride, box_cols, p.box_rows))
+      return fail(FA_ERR_CUDA, "cuTensorMapEncodeTiled failed for the KV cache");
+    const bool e4m3 = c.code == FA_CODE_E4M3;
+    auto* launch = P.hd == 64    ? (e4m3 ? launch_kv8_decode_64_e4m3 : launch_kv8_decode_64_int8)
+                   : P.hd == 128 ? (e4m3 ? launch_kv8_decode_128_e4m3 : launch_kv8_decode_128_int8)
+                                 : (e4m3 ? launch_kv8_decode_256_e4m3 : launch_kv8_decode_256_int8);
+    e = launch(P.wide, p, tm_k, tm_v, P.grid, st);
+  }
   if (e != cudaSuccess) return cuda_fail("attention kernel launch", e);
   count_launches(1);
   if (p.num_splits == 1) return FA_OK;
@@ -232,6 +239,7 @@ static int run_kv8_append(const fa_kv8_append_params& p_in, cudaStream_t st) {
       !ok8(p.vc_outer_stride) || !ok8(p.vc_row_stride) || !ok8(p.vc_head_stride))
     return fail(FA_ERR_UNSUPPORTED, "the codes of an 8-bit KV cache must start at 16-byte boundaries, with strides that are multiples of 16");
   if (p.total > 0x7fffffffLL || p.h_k > 65535) return fail(FA_ERR_UNSUPPORTED, "too many new tokens or heads in one call");
+  if ((int64_t)p.kv_outer * p.rows > 0x7fffffffLL) return fail(FA_ERR_UNSUPPORTED, "too many tokens in the KV cache");
   const int num_sm = p.num_sm > 0 ? p.num_sm : sm_count();
   int32_t* status = device_status_word();
   if (!status || num_sm <= 0) return fail(FA_ERR_CUDA, "cannot query the current device");

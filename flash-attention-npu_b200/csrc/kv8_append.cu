@@ -7,8 +7,10 @@
 // and otherwise its codes are rewritten in the new one; a run that starts at the block's first row starts the block afresh, so a
 // recycled page needs no clearing.  Rows behind the run are left alone.  Runs own their blocks: no atomics, no order to depend on.
 //
-// HBM-bound: 2 bytes an element in, 1 out.  A run's elements stay in registers between the maximum and the rounding (up to
-// kKeep 16-byte chunks a thread, the rest is read again), so everything is read once.
+// HBM-bound: 2 bytes an element in, 1 out.  A run's elements stay in registers between the maximum and the rounding, eight 16-byte chunks a
+// thread, so they are read once: a warp by itself writes a run of up to 256 chunks (16 tokens of head dim 128, and every
+// decoding token), the CTA's eight warps together one of up to 2048; what a longer run has beyond that is read twice.
+#include <algorithm>
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -16,7 +18,8 @@
 namespace fa {
 
 constexpr int kLeastScaleExp = 127 - 40;
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 256, kAppendWarps = kAppendThreads / 32;
+constexpr int kBatch = 8, kWarpRun = 32 * kBatch;
 
 // Bit pattern of the power of two above, from the largest |finite element| as an fp32 value.
 template <int CODE>
@@ -41,18 +44,6 @@ __device__ __forceinline__ uint32_t encode2(float a, float b) {
   return (uint32_t)(x & 255) | ((uint32_t)(y & 255) << 8);
 }
 
-// x / s, correctly rounded: by the reciprocal where that is exact.
-struct Divide {
-  float s, inv;
-  bool pow2;
-  __device__ __forceinline__ explicit Divide(float scale) : s(scale) {
-    const uint32_t u = __float_as_uint(scale);
-    pow2 = (u & 0x7fffffu) == 0 && (u >> 23) >= 1 && (u >> 23) <= 253;
-    inv = pow2 ? __uint_as_float((254u - (u >> 23)) << 23) : 0.f;
-  }
-  __device__ __forceinline__ float operator()(float x) const { return pow2 ? __fmul_rn(x, inv) : __fdiv_rn(x, s); }
-};
-
 template <typename T>
 __device__ __forceinline__ void unpack_pair(uint32_t w, float& a, float& b) {
   if (std::is_same<T, __nv_bfloat16>::value) {
@@ -64,59 +55,92 @@ __device__ __forceinline__ void unpack_pair(uint32_t w, float& a, float& b) {
     b = f.y;
   }
 }
-// Largest |element| bits of a pair among the finite ones, per half word.
+// Running maximum of |element| per half word; NaN has no part in it.
 template <typename T>
-__device__ __forceinline__ uint32_t finite_abs2(uint32_t w) {
-  constexpr uint32_t inf = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u;
-  const uint32_t a = w & 0x7fff7fffu;
-  return a & __vcmpltu2(a, inf);
+__device__ __forceinline__ uint32_t abs_max2(uint32_t mx, uint32_t w) {
+  w &= 0x7fff7fffu;
+  uint32_t r;
+  if (std::is_same<T, __nv_bfloat16>::value) asm("max.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
+  else asm("max.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
+  return r;
+}
+// A pair with its infinities taken out.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t inf = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+  return ((w & 0x7fffu) == inf ? 0u : w & 0xffffu) | (((w >> 16) & 0x7fffu) == inf ? 0u : w & 0xffff0000u);
 }
 
-// One run: `rows` tokens of `chunks` 16-byte chunks each into block rows first .. first + rows - 1.  GROUP threads work together
-// (a warp, or the whole CTA); `load(row, chunk)` gives a chunk of the source.
-template <typename T, int CODE, int GROUP, typename Load>
-__device__ __forceinline__ void write_run(Load load, uint8_t* block, int64_t row_stride, int first, int rows, int chunks, float* scale,
-                                          int t, float* s_red) {
-  constexpr int kKeep = 8;
-  const int n = rows * chunks;
-  uint4 keep[kKeep];
+// How GROUP threads share a run's 16-byte chunks: each has one column of every step-th row (what is left over idles).
+struct Share {
+  int col, row, step;
+  __device__ __forceinline__ Share(int t, int group, int chunks) {
+    step = group / chunks;
+    row = t / chunks;
+    col = t - row * chunks;
+    if (row >= step) row = 1 << 30;
+  }
+};
+
+// One run: `rows` tokens into block rows first .. first + rows - 1.  GROUP threads work together (a warp, or the whole CTA), t is
+// the thread among them; load(r): its column of new token r; dst: of the
+// block's first row.
+// BATCH: chunks of a thread that stay in registers; 1 is a short piece of code for runs of a token (a decoding step is over before the
+// instructions of the long one have arrived: 64 tokens 15.3 us with it alone).
+template <typename T, int CODE, int GROUP, int BATCH, typename Load>
+__device__ __forceinline__ void write_run(Load load, uint8_t* dst, int64_t row_stride, int first, int rows, const Share& my, float* scale, int t,
+                                          float* s_red) {
+  const float old = *scale;
+  uint4 keep[BATCH];
   uint32_t mx = 0;
+  auto fetch = [&](int r0) {
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k) {
-    const int c = t + k * GROUP;
-    keep[k] = make_uint4(0, 0, 0, 0);
-    if (c < n) keep[k] = load(c / chunks, c % chunks);
-  }
+    for (int k = 0; k < BATCH; ++k) {
+      keep[k] = make_uint4(0, 0, 0, 0);
+      if (r0 + k * my.step < rows) keep[k] = load(r0 + k * my.step);
+    }
+  };
+  const int more = BATCH * my.step;
+  for (int r0 = my.row + more; r0 < rows; r0 += more) {  // (the first batch last: it stays)
+    fetch(r0);
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(finite_abs2<T>(keep[k].x), finite_abs2<T>(keep[k].y)),
-                               __vmaxu2(finite_abs2<T>(keep[k].z), finite_abs2<T>(keep[k].w))));
-  for (int c = t + kKeep * GROUP; c < n; c += GROUP) {
-    const uint4 x = load(c / chunks, c % chunks);
-    mx = __vmaxu2(mx, __vmaxu2(__vmaxu2(finite_abs2<T>(x.x), finite_abs2<T>(x.y)), __vmaxu2(finite_abs2<T>(x.z), finite_abs2<T>(x.w))));
+    for (int k = 0; k < BATCH; ++k) mx = abs_max2<T>(abs_max2<T>(abs_max2<T>(abs_max2<T>(mx, keep[k].x), keep[k].y), keep[k].z), keep[k].w);
   }
+  fetch(my.row);
+#pragma unroll
+  for (int k = 0; k < BATCH; ++k) mx = abs_max2<T>(abs_max2<T>(abs_max2<T>(abs_max2<T>(mx, keep[k].x), keep[k].y), keep[k].z), keep[k].w);
   float lo, hi;
   unpack_pair<T>(mx, lo, hi);
+  if (fmaxf(lo, hi) == INFINITY) {  // rare: the maximum without the infinities
+    mx = 0;
+#pragma unroll 1
+    for (int r = my.row; r < rows; r += my.step) {
+      const uint4 x = load(r);
+      mx = abs_max2<T>(abs_max2<T>(mx, finite2<T>(x.x)), finite2<T>(x.y));
+      mx = abs_max2<T>(abs_max2<T>(mx, finite2<T>(x.z)), finite2<T>(x.w));
+    }
+    unpack_pair<T>(mx, lo, hi);
+  }
   float amax = fmaxf(lo, hi);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (GROUP > 32) {
-    __syncthreads();  // the run before this one has read s_red and the scale
+    __syncthreads();  // the run before this one has read s_red
     if ((t & 31) == 0) s_red[t >> 5] = amax;
-    __syncthreads();
+    __syncthreads();  // (everybody has read the old scale)
 #pragma unroll
     for (int w = 0; w < GROUP / 32; ++w) amax = fmaxf(amax, s_red[w]);
+  } else {
+    __syncwarp();
   }
-  const float need = pow2_scale<CODE>(amax), old = *scale;
+  const float need = pow2_scale<CODE>(amax);
   const float now = first == 0 ? need : fmaxf(old, need);
-  if (GROUP > 32) __syncthreads();
-  else __syncwarp();
   if (t == 0) *scale = now;
   if (first > 0 && now != old) {  // the block's scale has grown: its codes are written again
     const float ratio = __fdiv_rn(old, now);
-    const int held = first * chunks;
-    for (int c = t; c < held; c += GROUP) {
-      uint2* at = reinterpret_cast<uint2*>(block + (int64_t)(c / chunks) * row_stride + (c % chunks) * 8);
+#pragma unroll 1
+    for (int r = my.row; r < first; r += my.step) {
+      uint2* at = reinterpret_cast<uint2*>(dst + (int64_t)r * row_stride);
       uint2 w = *at;
       uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
@@ -130,8 +154,8 @@ __device__ __forceinline__ void write_run(Load load, uint8_t* block, int64_t row
       *at = w;
     }
   }
-  const Divide by(now);
-  auto store = [&](int c, const uint4& x) {
+  dst += (int64_t)first * row_stride;
+  auto put = [&](int r, const uint4& x, auto by) {  // by(x): x / now, correctly rounded
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
     uint32_t half[4];
 #pragma unroll
@@ -140,100 +164,120 @@ __device__ __forceinline__ void write_run(Load load, uint8_t* block, int64_t row
       unpack_pair<T>(w[e], a, b);
       half[e] = encode2<CODE>(by(a), by(b));
     }
-    *reinterpret_cast<uint2*>(block + (int64_t)(first + c / chunks) * row_stride + (c % chunks) * 8) =
-        make_uint2(half[0] | (half[1] << 16), half[2] | (half[3] << 16));
+    *reinterpret_cast<uint2*>(dst + (int64_t)r * row_stride) = make_uint2(half[0] | (half[1] << 16), half[2] | (half[3] << 16));
   };
+  const uint32_t bits = __float_as_uint(now), exponent = bits >> 23;
+  if ((bits & 0x7fffffu) == 0 && exponent >= 1 && exponent <= 253) {  // a power of two: its reciprocal is exact
+    const float inv = __uint_as_float((254u - exponent) << 23);
+    auto by = [&](float v) { return __fmul_rn(v, inv); };
+    for (int r0 = my.row;;) {
 #pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-    if (t + k * GROUP < n) store(t + k * GROUP, keep[k]);
-  for (int c = t + kKeep * GROUP; c < n; c += GROUP) store(c, load(c / chunks, c % chunks));
+      for (int k = 0; k < BATCH; ++k)
+        if (r0 + k * my.step < rows) put(r0 + k * my.step, keep[k], by);
+      r0 += more;
+      if (r0 >= rows) break;
+      fetch(r0);
+    }
+  } else {  // a scale that somebody else has chosen: rare, and kept short
+#pragma unroll 1
+    for (int r = my.row; r < rows; r += my.step) put(r, load(r), [&](float v) { return __fdiv_rn(v, now); });
+  }
 }
 
 // ---- packed tokens with a slot each ----
-// grid (token windows, kv heads, 2: K or V).  A CTA writes the runs that start in its window: those of up to kShortRun tokens a
-// warp each (a decoding step's tokens are runs of one), longer ones together.
-constexpr int kShortRun = 8, kMaxWindow = 32;
+// grid (windows of tokens, groups of (kv head, K or V) pairs).  A CTA lists the runs that start in its window and writes them for
+// its pairs: short ones a warp each, side by side, then the long ones together.
+constexpr int kMaxWindow = 256;
 
 template <typename T, int CODE>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const __grid_constant__ fa_kv8_append_params p, int window, int32_t* status) {
-  __shared__ float s_red[kAppendThreads / 32];
-  __shared__ int s_first[kMaxWindow], s_len[kMaxWindow];
-  __shared__ int64_t s_block[kMaxWindow];
+__global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(const __grid_constant__ fa_kv8_append_params p, int window, int32_t* status) {
+  __shared__ float s_red[kAppendWarps];
+  __shared__ int s_runs, s_tok[kMaxWindow], s_len[kMaxWindow];
+  __shared__ uint32_t s_slot[kMaxWindow];
   grid_wait();
-  const int tid = threadIdx.x, hk = blockIdx.y;
-  const bool is_v = blockIdx.z != 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t t0 = (int64_t)blockIdx.x * window;
-  const int sb = p.c.scale_block, chunks = p.d >> 3;
-  const int64_t slots = (int64_t)p.kv_outer * p.rows;
-  if (tid < window) {
-    const int64_t t = t0 + tid;
-    int len = 0;
-    int64_t blk = -1;
-    int row = 0;
-    if (t < p.total) {
-      const int64_t s = p.slots[t];
-      if (s >= slots) raise_bad_index(status);  // nowhere to write: skipped, like padding
-      if (s >= 0 && s < slots) {
-        blk = s / sb;
-        row = (int)(s - blk * sb);
-        // a run goes on while the slots follow one another within the block
-        const int64_t before = t > 0 ? p.slots[t - 1] : -1;
-        len = row == 0 || before != s - 1;
-      }
+  const uint32_t sb = (uint32_t)p.c.scale_block, blocks = (uint32_t)p.rows / sb;
+  const int64_t slots = (int64_t)p.kv_outer * p.rows;  // below 2^31
+  if (tid == 0) s_runs = 0;
+  __syncthreads();
+  if (tid < window && t0 + tid < p.total) {
+    const int64_t s = p.slots[t0 + tid], before = t0 + tid > 0 ? p.slots[t0 + tid - 1] : -1;
+    if (s >= slots) raise_bad_index(status);  // nowhere to write: skipped, like padding
+    if (s >= 0 && s < slots && (before != s - 1 || (uint32_t)s % sb == 0)) {  // a run starts
+      const int r = atomicAdd(&s_runs, 1);  // (in any order: runs do not know of one another)
+      s_tok[r] = tid;
+      s_slot[r] = (uint32_t)s;
     }
-    s_first[tid] = row;
-    s_len[tid] = len;
-    s_block[tid] = blk;
   }
   __syncthreads();
-  for (int w = tid >> 5; w < window; w += kAppendThreads / 32) {  // lengths of the runs that start here, 32 tokens at a time
-    if (s_len[w] == 0) continue;
-    const int64_t t = t0 + w, s = s_block[w] * sb + s_first[w];
-    const int most = (int)min((int64_t)(sb - s_first[w]), p.total - t), lane = tid & 31;
-    int len = 0;
-    for (;;) {
-      const int i = len + lane;
-      const unsigned off = __ballot_sync(0xffffffffu, i >= most || p.slots[t + i] != s + i);
-      if (off) {
-        len += __ffs(off) - 1;
-        break;
+  const int runs = s_runs;
+  for (int r = warp; r < runs; r += kAppendWarps) {  // it goes on while the slots follow one another within the block
+    const int64_t t = t0 + s_tok[r], s = s_slot[r];
+    const int most = (int)min((int64_t)(sb - (uint32_t)s % sb), p.total - t);
+    int len = 0, more = 0;
+    do {
+      bool on[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = len + 32 * k + lane;
+        on[k] = i < most && p.slots[t + i] == s + i;
       }
-      len += 32;
-    }
-    __syncwarp();
-    if (lane == 0) s_len[w] = len;
+      more = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned off = ~__ballot_sync(0xffffffffu, on[k]);
+        if (more == 32 * k) more += off ? __ffs(off) - 1 : 32;
+      }
+      len += more;
+    } while (more == 128);
+    if (lane == 0) s_len[r] = len;
   }
   __syncthreads();
-  const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)hk * (is_v ? p.v_head_stride : p.k_head_stride);
-  const int64_t tok_stride = is_v ? p.v_tok_stride : p.k_tok_stride;
-  uint8_t* codes = reinterpret_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + (int64_t)hk * (is_v ? p.vc_head_stride : p.kc_head_stride);
-  const int64_t outer_stride = is_v ? p.vc_outer_stride : p.kc_outer_stride, row_stride = is_v ? p.vc_row_stride : p.kc_row_stride;
-  float* scale = (is_v ? p.c.v_scale : p.c.k_scale) + (int64_t)hk * (is_v ? p.c.vs_head_stride : p.c.ks_head_stride);
-  const int64_t so = is_v ? p.c.vs_outer_stride : p.c.ks_outer_stride, sbs = is_v ? p.c.vs_block_stride : p.c.ks_block_stride;
-  const int blocks = p.rows / sb;
-  auto run = [&](auto group, int w, int t) {
-    constexpr int GROUP = decltype(group)::value;
-    const int64_t blk = s_block[w], outer = blk / blocks;
-    const int in = (int)(blk - outer * blocks);
-    const T* x = src + (t0 + w) * tok_stride;
-    auto load = [&](int r, int c) { return *reinterpret_cast<const uint4*>(x + (int64_t)r * tok_stride + c * 8); };
-    write_run<T, CODE, GROUP>(load, codes + outer * outer_stride + (int64_t)in * sb * row_stride, row_stride, s_first[w], s_len[w], chunks,
-                              scale + outer * so + (int64_t)in * sbs, t, s_red);
+  const int chunks = p.d >> 3;
+  const Share alone(lane, 32, chunks), together(tid, kAppendThreads, chunks);
+  auto run = [&](auto group, auto batch, int r, int pair, int t) {
+    const int hk = pair >> 1;
+    const bool is_v = pair & 1;
+    const uint32_t s = s_slot[r], blk = s / sb, outer = blk / blocks, in = blk - outer * blocks;
+    const int64_t tok = is_v ? p.v_tok_stride : p.k_tok_stride, row_stride = is_v ? p.vc_row_stride : p.kc_row_stride;
+    const T* x = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)hk * (is_v ? p.v_head_stride : p.k_head_stride) + (t0 + s_tok[r]) * tok;
+    uint8_t* codes = reinterpret_cast<uint8_t*>(is_v ? p.v_cache : p.k_cache) + (int64_t)hk * (is_v ? p.vc_head_stride : p.kc_head_stride) +
+                     outer * (is_v ? p.vc_outer_stride : p.kc_outer_stride) + (int64_t)(in * sb) * row_stride;
+    float* scale = is_v ? p.c.v_scale + hk * p.c.vs_head_stride + outer * p.c.vs_outer_stride + in * p.c.vs_block_stride
+                        : p.c.k_scale + hk * p.c.ks_head_stride + outer * p.c.ks_outer_stride + in * p.c.ks_block_stride;
+    const Share& my = decltype(group)::value == 32 ? alone : together;
+    x += my.col * 8;
+    auto load = [&](int row) { return *reinterpret_cast<const uint4*>(x + (int64_t)row * tok); };
+    write_run<T, CODE, decltype(group)::value, decltype(batch)::value>(load, codes + my.col * 8, row_stride, (int)(s % sb), s_len[r], my, scale, t, s_red);
   };
-  for (int w = tid >> 5; w < window; w += kAppendThreads / 32)
-    if (s_len[w] > 0 && s_len[w] <= kShortRun) run(std::integral_constant<int, 32>(), w, tid & 31);
-  for (int w = 0; w < window; ++w)
-    if (s_len[w] > kShortRun) run(std::integral_constant<int, kAppendThreads>(), w, tid);
+  using std::integral_constant;
+  const int pairs = 2 * p.h_k;
+  const int mine = (pairs - blockIdx.y + gridDim.y - 1) / gridDim.y;  // every gridDim.y-th pair
+  for (int i = warp; i < runs * mine; i += kAppendWarps) {
+    const int m = i / runs, r = i - m * runs, pair = blockIdx.y + m * gridDim.y, n = s_len[r] * chunks;
+    if (n <= 32) run(integral_constant<int, 32>(), integral_constant<int, 1>(), r, pair, lane);
+    else if (n <= kWarpRun) run(integral_constant<int, 32>(), integral_constant<int, kBatch>(), r, pair, lane);
+  }
+  for (int r = 0; r < runs; ++r) {
+    if (s_len[r] * chunks <= kWarpRun) continue;
+    for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y)
+      run(integral_constant<int, kAppendThreads>(), integral_constant<int, kBatch>(), r, pair, tid);
+  }
 }
 
 // ---- new tokens of an attention call: (b, s_new, h_k, d) behind cache_seqlens, k rotated when rotary tables are given ----
-// grid (blocks that a sequence can touch x b, kv heads, 2).
-template <typename T, int CODE, int GROUP>
-__global__ void __launch_bounds__(GROUP) kv8_append_dense_kernel(const __grid_constant__ Kv8Params p, int touched) {
-  __shared__ float s_red[GROUP / 32];
+// Units (touched block of a sequence, kv head, K or V), GROUP threads each; BATCH as above.
+template <typename T, int CODE, int GROUP, int BATCH>
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_dense_kernel(const __grid_constant__ Kv8Params p, int touched, int units) {
+  __shared__ float s_red[kAppendWarps];
   grid_wait();
-  const int bi = blockIdx.x / touched, nth = blockIdx.x - bi * touched, hk = blockIdx.y, tid = threadIdx.x;
-  const bool is_v = blockIdx.z != 0;
+  const int tid = threadIdx.x;
+  const int unit = GROUP == 32 ? blockIdx.x * kAppendWarps + (tid >> 5) : blockIdx.x;
+  if (unit >= units) return;
+  const int pairs = 2 * p.a.h_k, seq = unit / pairs, pair = unit - seq * pairs, hk = pair >> 1;
+  const int bi = seq / touched, nth = seq - bi * touched;
+  const bool is_v = pair & 1;
   const int len = cache_len(p.a, bi, p.status), sb = p.c.scale_block;
   const int blk = len / sb + nth;  // of the sequence
   const int lo = max(len, blk * sb), hi = min(len + p.a.seqlen_new, (blk + 1) * sb);
@@ -264,7 +308,9 @@ __global__ void __launch_bounds__(GROUP) kv8_append_dense_kernel(const __grid_co
   float* scale = is_v ? p.c.v_scale + outer * p.c.vs_outer_stride + (int64_t)(row / sb) * p.c.vs_block_stride + hk * p.c.vs_head_stride
                       : p.c.k_scale + outer * p.c.ks_outer_stride + (int64_t)(row / sb) * p.c.ks_block_stride + hk * p.c.ks_head_stride;
   const bool rotate = !is_v && p.a.rotary_cos != nullptr;
-  auto load = [&](int r, int c) {
+  const Share my(GROUP == 32 ? (tid & 31) : tid, GROUP, p.a.d >> 3);
+  const int c = my.col;
+  auto load = [&](int r) {
     const T* xr = x + (int64_t)(lo - len + r) * tok;
     uint4 v = *reinterpret_cast<const uint4*>(xr + c * 8);
     if (rotate) {
@@ -275,16 +321,18 @@ __global__ void __launch_bounds__(GROUP) kv8_append_dense_kernel(const __grid_co
     }
     return v;
   };
-  write_run<T, CODE, GROUP>(load, codes, row_stride, lo - blk * sb, hi - lo, p.a.d >> 3, scale, tid, s_red);
+  write_run<T, CODE, GROUP, BATCH>(load, codes + c * 8, row_stride, lo - blk * sb, hi - lo, my, scale, GROUP == 32 ? (tid & 31) : tid, s_red);
 }
 
 template <typename T, int CODE>
 static cudaError_t append_t(const fa_kv8_append_params& p, int num_sm, int32_t* status, cudaStream_t st) {
-  // Windows of as many tokens as leave every SM eight CTAs: a window of one token finds a decoding step's runs side by side, a
-  // longer one spares the CTAs in which no run of a prompt starts.
-  int64_t w = p.total * p.h_k * 2 / (8LL * num_sm);
-  const int window = (int)(w < 1 ? 1 : w > kMaxWindow ? kMaxWindow : w);
-  const dim3 grid((unsigned)((p.total + window - 1) / window), (unsigned)p.h_k, 2);
+  // A window has as many tokens as leave every SM eight CTAs, up to a scale block, in which one run of a prompt starts: one for a
+  // decoding step, whose runs then lie side by side.  A CTA has one pair for long runs, eight for warps that write alone.
+  const int pairs = 2 * p.h_k, sb = p.c.scale_block;
+  const int groups = std::min<int64_t>(p.total, sb) * (p.d / 8) > kWarpRun ? pairs : (pairs + kAppendWarps - 1) / kAppendWarps;
+  const int most = std::min(kMaxWindow, sb);
+  const int window = (int)std::min<int64_t>(most, std::max<int64_t>(1, p.total * groups / (8LL * num_sm)));
+  const dim3 grid((unsigned)((p.total + window - 1) / window), (unsigned)groups);
   return launch_dependent(kv8_append_kernel<T, CODE>, grid, kAppendThreads, 0, st, p, window, status);
 }
 cudaError_t launch_kv8_append(const fa_kv8_append_params& p, int num_sm, int32_t* status, cudaStream_t st) {
@@ -296,10 +344,12 @@ cudaError_t launch_kv8_append(const fa_kv8_append_params& p, int num_sm, int32_t
 
 template <typename T, int CODE>
 static cudaError_t append_dense_t(const Kv8Params& p, cudaStream_t st) {
-  const int sb = p.c.scale_block, touched = (p.a.seqlen_new + sb - 2) / sb + 1;
-  const dim3 grid((unsigned)(touched * p.a.b), (unsigned)p.a.h_k, 2);
-  if (p.a.seqlen_new <= kShortRun) return launch_dependent(kv8_append_dense_kernel<T, CODE, 32>, grid, 32, 0, st, p, touched);
-  return launch_dependent(kv8_append_dense_kernel<T, CODE, kAppendThreads>, grid, kAppendThreads, 0, st, p, touched);
+  const int sb = p.c.scale_block, touched = (p.a.seqlen_new + sb - 2) / sb + 1, units = touched * p.a.b * 2 * p.a.h_k;
+  const int n = std::min(sb, p.a.seqlen_new) * (p.a.d / 8);
+  const dim3 one((unsigned)units), eight((unsigned)ceil_div(units, kAppendWarps));  // units a CTA
+  if (n <= 32) return launch_dependent(kv8_append_dense_kernel<T, CODE, 32, 1>, eight, kAppendThreads, 0, st, p, touched, units);
+  if (n <= kWarpRun) return launch_dependent(kv8_append_dense_kernel<T, CODE, 32, kBatch>, eight, kAppendThreads, 0, st, p, touched, units);
+  return launch_dependent(kv8_append_dense_kernel<T, CODE, kAppendThreads, kBatch>, one, kAppendThreads, 0, st, p, touched, units);
 }
 cudaError_t launch_kv8_append_dense(const Kv8Params& p, cudaStream_t st) {
   if (p.a.dtype == FA_BF16)

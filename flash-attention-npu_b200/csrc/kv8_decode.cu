@@ -1,7 +1,7 @@
-// Host side of the 8-bit decode kernel: tile facts and tensor maps.
+// Tile facts of the 8-bit kernels for the host planner.
 #include "kv8_api.cuh"
 #include "kv8_decode_kernel.cuh"
-#include "tc5_api.cuh"
+#include "kv8_tile_kernel.cuh"
 
 namespace fa {
 
@@ -12,6 +12,13 @@ Kv8TileInfo kv8_decode_info(int hd, bool wide) {
   if (hd == 64) return wide ? info<Kv8Traits<64, 2>>() : info<Kv8Traits<64, 1>>();
   if (hd == 128) return wide ? info<Kv8Traits<128, 2>>() : info<Kv8Traits<128, 1>>();
   return wide ? info<Kv8Traits<256, 2>>() : info<Kv8Traits<256, 1>>();
+}
+
+template <class Tr>
+static Kv8TileInfo tile_info() { return Kv8TileInfo{Tr::BM, Tr::BN, Tr::NTHREADS, Tr::SMEM_BYTES, 1}; }
+
+Kv8TileInfo kv8_tile_info(int hd) {
+  return hd == 64 ? tile_info<Kv8TileTraits<64>>() : hd == 128 ? tile_info<Kv8TileTraits<128>>() : tile_info<Kv8TileTraits<256>>();
 }
 
 }  // namespace fa

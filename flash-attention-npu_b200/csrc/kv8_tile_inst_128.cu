@@ -1,0 +1,3 @@
+#define FA_INST_HD 128
+#define FA_INST_NAME launch_kv8_tile_128
+#include "kv8_tile_inst.inc"

@@ -1,0 +1,3 @@
+#define FA_INST_HD 64
+#define FA_INST_NAME launch_kv8_tile_64
+#include "kv8_tile_inst.inc"

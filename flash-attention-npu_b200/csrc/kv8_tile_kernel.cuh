@@ -1,0 +1,584 @@
+// Attention over an 8-bit KV cache for many query rows: tcgen05 products with accumulators in TMEM, fp16 operands.
+//
+// A CTA has a tile of packed query rows (row = token * group + head; all heads of a kv head's group, so a key is turned into fp16
+// once for all of them) against a range of key blocks; ranges are cut where the tiles are too few for the chip (kv8_api.cu).
+// Arithmetic as in kv8_decode_kernel.cuh: V's scale in the exponent, P' in fp16, scales never in a product.  The reference m of
+// the exponent is the running maximum, moved only when that has grown by more than 2^8: P' = 2^(x - m + 7) stays below 2^15, far from
+// fp16's end, and below 2^7 it has as many bits as a 16-bit output shows; so O is rescaled in TMEM a few times a tile and
+// not at every block.
+//
+// Warps: 4 per sub-tile of 128 rows  softmax, one thread per row (Q load, P, rescale of O, epilogue)
+//        4                           converters: codes -> fp16 tiles in the swizzled operand layout; global loads of a tile in flight
+//                                    while the one before is turned
+//        1 per sub-tile              MMA issue
+// Head dims up to 128: two sub-tiles, whose softmax and products alternate; S0 S1 O0 O1 fill TMEM.  256 columns: one sub-tile
+// with two buffers of S and P for blocks of 64 keys.
+//
+// Bound: per 128 keys and 256 rows of head dim 128 the products take 2048 cycles of an SM's tensor pipe, the exponentials 2048 of its
+// special-function unit, turning the codes about 1000 of its 8192 issue slots.  TMA cannot convert, so the codes pass through registers.
+#pragma once
+
+#include <type_traits>
+
+#include "kv8.cuh"
+
+namespace fa {
+
+template <int HD_>
+struct Kv8TileTraits {
+  static constexpr int HD = HD_;
+  static constexpr int NSUB = HD <= 128 ? 2 : 1, SB = 3 - NSUB;  // sub-tiles; S / P buffers of each
+  static constexpr int BM = 128 * NSUB, BN = HD <= 128 ? 128 : 64;
+  static constexpr int GROUPS = BN / kScaleGranule;
+  static constexpr int HALVES = HD / 64;                 // 64-column halves of Q, K, V
+  static constexpr int KV_HALF = BN * 128, SLOT_BYTES = HALVES * KV_HALF;
+  static constexpr int Q_HALF = 128 * 128, Q_BYTES = HALVES * Q_HALF;  // per sub-tile
+  static constexpr int P_HALF = 128 * 128, P_BYTES = BN / 64 * P_HALF; // per sub-tile and buffer
+  static constexpr int RING = HD == 128 ? 3 : 4;
+  static constexpr int Q_OFF = 0, P_OFF = NSUB * Q_BYTES, RING_OFF = P_OFF + NSUB * SB * P_BYTES, TAIL_OFF = RING_OFF + RING * SLOT_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + TAIL_OFF;
+  static constexpr int SOFTMAX_WARPS = 4 * NSUB, CONV_WARPS = 4, NTHREADS = 32 * (SOFTMAX_WARPS + CONV_WARPS + NSUB);
+  static constexpr int CPR = HD / 16, CHUNKS = BN * CPR / 128;  // 16-code chunks of a key row; of a converter thread in a tile
+  static constexpr int O_COL = 256, O_STEP = 128, S_STEP = NSUB == 2 ? 128 : BN;  // TMEM columns
+  static constexpr int SCR = 4;  // blocks of scales in flight
+};
+
+struct Kv8TileShared {
+  uint64_t q_full[2], kv_full[4], kv_empty[4];
+  uint64_t s_full[2][2], s_free[2][2];  // [sub-tile][buffer]
+  uint64_t p_full[2][2], pv_done[2][2];
+  uint64_t sc_full[4], sc_empty[4];
+  float sc[4][3][8];  // of a block: score factor, log2 of V's scale, its reciprocal, per 16 keys
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// Ring positions in the order the products need the tiles: K_0 | K_1 V_0 | K_2 V_1 | ... | V_last.
+template <int SLOTS>
+struct Kv8Ring {
+  uint32_t at = 0, phase = 0;
+  __device__ __forceinline__ void next(uint32_t& slot, uint32_t& par) {
+    slot = at;
+    par = phase;
+    if (++at == SLOTS) { at = 0; phase ^= 1; }
+  }
+};
+
+// ---------------- converters ----------------
+template <class Tr, int CODE>
+__device__ __forceinline__ void kv8_convert(const Kv8Params& p, const Kv8Seq& sq, const Kv8Seg& sg, Kv8TileShared* sh, uint32_t ring_smem,
+                                            float mul, int tid) {
+  constexpr int NC = Tr::CHUNKS, CPR = Tr::CPR;
+  volatile int* abort_flag = &sh->abort_flag;
+  const int lane = tid & 31, warp = tid >> 5;
+  const int c16 = tid % CPR, row0 = tid / CPR;  // this thread's chunk column, first row; rows advance by 128 / CPR
+  const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.a.k) + (int64_t)sg.hk * p.a.k_head_stride + c16 * 16;
+  const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.a.v) + (int64_t)sg.hk * p.a.v_head_stride + c16 * 16;
+  const bool col_on = c16 * 16 < p.a.d;
+
+  // lane g: page (or cache row) and row in it of the block's 16-key group g; looked up only where a row sees one of its keys
+  struct Where { int outer, row; };
+  auto locate = [&](int it) {
+    const int t = (sg.lo + it) * Tr::BN + lane * kScaleGranule;
+    Where w{0, -1};
+    if (it < sg.cnt && lane < Tr::GROUPS && t < sq.key_hi && t + kScaleGranule > sq.key_lo) {
+      w.outer = sq.batch_row;
+      w.row = t;
+      if (sq.pages) {
+        const int pg = t / p.a.page_size;
+        w.row = t - pg * p.a.page_size;
+        const int id = __ldg(sq.pages + pg);
+        w.outer = outer_index(p.a, id, p.status);
+        if (id != w.outer) w.row = -1;  // not there: zeros
+      }
+    }
+    return w;
+  };
+  auto fetch = [&](uint4 (&x)[NC], const Where& w, int it, bool is_v) {
+    const int t0 = (sg.lo + it) * Tr::BN;
+    const uint8_t* base = is_v ? vb : kb;
+    const int64_t os = is_v ? p.a.v_batch_stride : p.a.k_batch_stride, rs = is_v ? p.a.v_row_stride : p.a.k_row_stride;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int row = row0 + i * (128 / CPR), g = row / kScaleGranule;
+      const int outer = __shfl_sync(0xffffffffu, w.outer, g), r = __shfl_sync(0xffffffffu, w.row, g);
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (r >= 0 && col_on && t0 + row >= sq.key_lo && t0 + row < sq.key_hi)
+        x[i] = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)outer * os + (int64_t)(r + row % kScaleGranule) * rs));
+    }
+  };
+  // scales of a block: lanes 0 .. GROUPS - 1 of warp 0 K's, the next ones V's
+  auto fetch_scale = [&](const Where& w) {
+    const int g = lane % Tr::GROUPS;
+    const int outer = __shfl_sync(0xffffffffu, w.outer, g), r = __shfl_sync(0xffffffffu, w.row, g);
+    if (r < 0 || lane >= 2 * Tr::GROUPS) return 0.f;
+    const int64_t blk = r / p.c.scale_block;
+    return lane < Tr::GROUPS ? __ldg(p.c.k_scale + outer * p.c.ks_outer_stride + blk * p.c.ks_block_stride + sg.hk * p.c.ks_head_stride)
+                             : __ldg(p.c.v_scale + outer * p.c.vs_outer_stride + blk * p.c.vs_block_stride + sg.hk * p.c.vs_head_stride);
+  };
+
+  Kv8Ring<Tr::RING> ring;
+  auto put = [&](const uint4 (&x)[NC]) {
+    uint32_t slot, par;
+    ring.next(slot, par);
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->kv_empty[slot]), par ^ 1, abort_flag, 71)) return false;
+    const uint32_t tile = ring_smem + slot * Tr::SLOT_BYTES + (c16 >> 2) * Tr::KV_HALF;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int row = row0 + i * (128 / CPR);
+      uint32_t h[8];
+      decode4<CODE>(x[i].x, h[0], h[1]);
+      decode4<CODE>(x[i].y, h[2], h[3]);
+      decode4<CODE>(x[i].z, h[4], h[5]);
+      decode4<CODE>(x[i].w, h[6], h[7]);
+      // lanes of odd halves store their second 8 columns first: the eight lanes of a row then meet eight different banks
+      const bool swap = (c16 >> 2) & 1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool second = (e == 1) != swap;
+        const uint32_t at = tile + row * 128 + ((((c16 & 3) * 2 + (second ? 1 : 0)) ^ (row & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(second ? h[4] : h[0]), "r"(second ? h[5] : h[1]),
+                     "r"(second ? h[6] : h[2]), "r"(second ? h[7] : h[3])
+                     : "memory");
+      }
+    }
+    tc5::fence_proxy_async();  // generic-proxy stores -> visible to the MMA
+    __syncwarp();
+    if (lane == 0) tc5::mbar_arrive(tc5::smem_addr(&sh->kv_full[slot]));
+    return true;
+  };
+  auto put_scale = [&](int it, float s) {
+    if (warp != 0) return true;
+    const int e = it % Tr::SCR;
+    if (it >= Tr::SCR && !tc5::mbar_wait(tc5::smem_addr(&sh->sc_empty[e]), (it / Tr::SCR - 1) & 1, abort_flag, 72)) return false;
+    if (lane < Tr::GROUPS) {
+      sh->sc[e][0][lane] = s * mul;
+    } else if (lane < 2 * Tr::GROUPS) {
+      const float v = usable_scale(s);
+      sh->sc[e][1][lane - Tr::GROUPS] = log2f(v);
+      sh->sc[e][2][lane - Tr::GROUPS] = 1.f / v;
+    }
+    __syncwarp();
+    if (lane == 0) tc5::mbar_arrive(tc5::smem_addr(&sh->sc_full[e]));
+    return true;
+  };
+
+  // Tiles in ring order, one ahead in registers; the pages of a block are looked up a block before its K is wanted.
+  struct Tile { bool k; int it; };
+  int kq = 0, vq = 0;
+  Where w0 = locate(0), w1 = locate(1), w2 = locate(2);  // of blocks vq, vq + 1, vq + 2
+  auto load = [&](uint4 (&x)[NC], float& s, Tile& tile) {
+    if (vq == sg.cnt) return false;
+    if (kq < sg.cnt && kq <= vq + 1) {
+      const Where w = kq == vq ? w0 : w1;
+      tile = Tile{true, kq};
+      fetch(x, w, kq, false);
+      s = fetch_scale(w);
+      ++kq;
+    } else {
+      tile = Tile{false, vq};
+      fetch(x, w0, vq, true);
+      ++vq;
+      w0 = w1;
+      w1 = w2;
+      w2 = locate(vq + 2);
+    }
+    return true;
+  };
+  auto emit = [&](const uint4 (&x)[NC], float s, const Tile& tile) { return (!tile.k || put_scale(tile.it, s)) && put(x); };
+  uint4 xa[NC], xb[NC];
+  float sa = 0.f, sb = 0.f;
+  Tile ta{}, tb{};
+  bool more = load(xa, sa, ta);
+  while (more) {
+    more = load(xb, sb, tb);
+    if (!emit(xa, sa, ta) || !more) return;
+    more = load(xa, sa, ta);
+    if (!emit(xb, sb, tb)) return;
+  }
+}
+
+// ---------------- MMA issue, sub-tile t ----------------
+template <class Tr>
+__device__ __forceinline__ void kv8_issue(Kv8TileShared* sh, uint32_t smem, uint32_t tmem, int t, int cnt) {
+  volatile int* abort_flag = &sh->abort_flag;
+  constexpr uint32_t idesc_qk = tc5::make_idesc(0, 128, Tr::BN, 0), idesc_pv = tc5::make_idesc(0, 128, Tr::HD, 1);
+  const uint64_t q_desc = tc5::make_smem_desc(smem + Tr::Q_OFF + t * Tr::Q_BYTES, 16, 1024);
+  const uint64_t p_desc0 = tc5::make_smem_desc(smem + Tr::P_OFF + t * Tr::SB * Tr::P_BYTES, 16, 1024);
+  const uint64_t k_desc0 = tc5::make_smem_desc(smem + Tr::RING_OFF, 16, 1024);            // K-major
+  const uint64_t v_desc0 = tc5::make_smem_desc(smem + Tr::RING_OFF, Tr::KV_HALF, 1024);   // N-contiguous
+  constexpr uint64_t kSlot = Tr::SLOT_BYTES >> 4;
+  // 16 columns per k-step = 32 bytes inside the 128-byte swizzle span
+  auto off = [](int ks, int half) { return (uint64_t)(((ks >> 2) * half + (ks & 3) * 32) >> 4); };
+  const uint32_t o_tmem = tmem + Tr::O_COL + t * Tr::O_STEP;
+  Kv8Ring<Tr::RING> ring;
+  if (!tc5::mbar_wait(tc5::smem_addr(&sh->q_full[t]), 0, abort_flag, 73)) return;
+  // a ring slot is free when the products of every sub-tile that has rows have read it
+  auto release = [&](uint32_t slot) { tc5::mma_commit(tc5::smem_addr(&sh->kv_empty[slot])); };
+  auto qk = [&](int it) {
+    uint32_t slot, par;
+    ring.next(slot, par);
+    const int b = it % Tr::SB;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->kv_full[slot]), par, abort_flag, 74)) return false;
+    if (it >= Tr::SB && !tc5::mbar_wait(tc5::smem_addr(&sh->s_free[t][b]), (it / Tr::SB - 1) & 1, abort_flag, 75)) return false;
+    tc5::tc_fence_after();
+    const uint64_t k_desc = k_desc0 + slot * kSlot;
+    const uint32_t s_tmem = tmem + (Tr::NSUB == 2 ? t : b) * Tr::S_STEP;
+    if (tc5::elect_one()) {
+      tc5::mma_ss_c<false>(s_tmem, q_desc, k_desc, idesc_qk);
+#pragma unroll
+      for (int ks = 1; ks < Tr::HD / 16; ++ks) tc5::mma_ss_c<true>(s_tmem, q_desc + off(ks, Tr::Q_HALF), k_desc + off(ks, Tr::KV_HALF), idesc_qk);
+      tc5::mma_commit(tc5::smem_addr(&sh->s_full[t][b]));
+      release(slot);
+    }
+    __syncwarp();
+    return true;
+  };
+  auto pv = [&](int it) {
+    uint32_t slot, par;
+    ring.next(slot, par);
+    const int b = it % Tr::SB;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->kv_full[slot]), par, abort_flag, 76)) return false;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->p_full[t][b]), (it / Tr::SB) & 1, abort_flag, 77)) return false;
+    tc5::tc_fence_after();
+    const uint64_t v_desc = v_desc0 + slot * kSlot, p_desc = p_desc0 + b * (uint64_t)(Tr::P_BYTES >> 4);
+    if (tc5::elect_one()) {
+      if (it == 0) tc5::mma_ss_c<false>(o_tmem, p_desc, v_desc, idesc_pv);
+      else tc5::mma_ss_c<true>(o_tmem, p_desc, v_desc, idesc_pv);
+#pragma unroll
+      for (int ks = 1; ks < Tr::BN / 16; ++ks)
+        tc5::mma_ss_c<true>(o_tmem, p_desc + off(ks, Tr::P_HALF), v_desc + (uint64_t)(ks * (2048 >> 4)), idesc_pv);
+      tc5::mma_commit(tc5::smem_addr(&sh->pv_done[t][b]));
+      release(slot);
+    }
+    __syncwarp();
+    return true;
+  };
+  if (!qk(0)) return;
+  for (int it = 0; it < cnt; ++it) {
+    if (it + 1 < cnt && !qk(it + 1)) return;
+    if (!pv(it)) return;
+  }
+}
+
+// ---------------- softmax, one thread per row ----------------
+template <class Tr, typename T, bool CAP>
+__device__ __forceinline__ void kv8_softmax(const Kv8Params& p, const Kv8Mask& mask, const Kv8Seq& sq, const Kv8Seg& sg, Kv8TileShared* sh,
+                                            uint32_t smem, uint32_t tmem, int t, int lane_row) {
+  volatile int* abort_flag = &sh->abort_flag;
+  const int lane = lane_row & 31, warp = lane_row >> 5;
+  const int rr = sg.mb * Tr::BM + t * 128 + lane_row, rows_total = sq.q_len * p.group;
+  const bool live = rr < rows_total;
+  const int i = rr / p.group, head = sg.hk * p.group + (rr - i * p.group);
+  // ---- Q: fp16, negated for a negative scale (scores then grow with the products), bf16 rows brought into fp16's range ----
+  float back = 1.f;
+  {
+    const uint32_t q_smem = smem + Tr::Q_OFF + t * Tr::Q_BYTES + lane_row * 128;
+    const T* qrow = reinterpret_cast<const T*>(p.a.q) + (int64_t)sg.bi * p.a.q_batch_stride + (int64_t)(sq.q_row0 + i) * p.a.q_row_stride +
+                    (int64_t)head * p.a.q_head_stride;
+    const bool rot = mask.causal || mask.local;
+    float up = 1.f;
+    if (std::is_same<T, __nv_bfloat16>::value) {
+      uint32_t mx = 0;
+      if (live) {
+#pragma unroll 4
+        for (int c8 = 0; c8 < p.a.d; c8 += 8) {
+          const uint4 x = kv8_q_chunk<T>(p, qrow, c8, sq.k_len, i, rot);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
+            mx = max(mx, max(w & 0x7fffu, (w >> 16) & 0x7fffu));
+          }
+        }
+      }
+      back = bf16_row_factor(mx, up);
+    }
+    const float sign = p.a.softmax_scale < 0.f ? -1.f : 1.f;
+    up *= sign;
+#pragma unroll 2
+    for (int ch = 0; ch < Tr::HD / 8; ++ch) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (live && ch * 8 < p.a.d) x = kv8_q_chunk<T>(p, qrow, ch * 8, sq.k_len, i, rot);
+      uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      if (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack2<__half>(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xffff0000u) * up);
+      } else if (sign < 0.f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] ^= 0x80008000u;
+      }
+      const uint32_t at = q_smem + (ch >> 3) * Tr::Q_HALF + (((ch & 7) ^ (lane_row & 7)) << 4);
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+    tc5::fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) tc5::mbar_arrive(tc5::smem_addr(&sh->q_full[t]));
+  }
+  // ---- what the row sees ----
+  int row_lo = 0, row_hi = sq.k_len - 1;
+  if (mask.causal) row_hi = min(row_hi, i + sq.koff);
+  if (mask.local) {
+    row_hi = min(row_hi, i + sq.koff + mask.wr);
+    row_lo = max(0, i + sq.koff - mask.wl);
+  }
+  if (!live) row_hi = -1;
+  // ... and every row of the warp: keys [all_lo, all_hi)
+  const int all_lo = __reduce_max_sync(0xffffffffu, live ? row_lo : 0), all_hi = __reduce_min_sync(0xffffffffu, live ? row_hi + 1 : 0x7fffffff);
+  const bool any_live = __any_sync(0xffffffffu, live);
+  const float cap_l2 = p.a.softcap * kLog2e;
+  const uint32_t lane_base = (uint32_t)warp << 21;  // 32 TMEM lanes a warp
+  const uint32_t o_tmem = tmem + Tr::O_COL + t * Tr::O_STEP + lane_base;
+  float m_ref = -INFINITY, m_run = -INFINITY, l = 0.f;
+
+  for (int it = 0; it < sg.cnt; ++it) {
+    const int b = it % Tr::SB, e = it % Tr::SCR, t0 = (sg.lo + it) * Tr::BN;
+    const uint32_t s_tmem = tmem + (Tr::NSUB == 2 ? t : b) * Tr::S_STEP + lane_base;
+    const uint32_t p_smem = smem + Tr::P_OFF + (t * Tr::SB + b) * Tr::P_BYTES + lane_row * 128;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->sc_full[e]), (it / Tr::SCR) & 1, abort_flag, 78)) return;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->s_full[t][b]), (it / Tr::SB) & 1, abort_flag, 79)) return;
+    tc5::tc_fence_after();
+    const bool edge = t0 < all_lo || t0 + Tr::BN > all_hi;
+    if (any_live) {
+      // ---- maximum ----
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < Tr::BN / 32; ++c) {
+        uint32_t r[32];
+        tc5::tmem_ld32(s_tmem + c * 32, r);
+        tc5::tmem_wait_ld();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float x[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            x[k] = __uint_as_float(r[g * 16 + k]);
+            if (edge) {
+              const int j = t0 + c * 32 + g * 16 + k;
+              if (j < row_lo || j > row_hi) x[k] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int s = 8; s > 0; s >>= 1)
+#pragma unroll
+            for (int k = 0; k < s; ++k) x[k] = fmaxf(x[k], x[k + s]);
+          const float c1 = sh->sc[e][0][c * 2 + g] * back, lv = sh->sc[e][1][c * 2 + g];
+          float xm;
+          if (CAP) {
+            const float ex = __expf(2.f * (x[0] * c1));
+            xm = x[0] == -INFINITY ? -INFINITY : cap_l2 * (1.f - __fdividef(2.f, ex + 1.f)) + lv;
+          } else {
+            xm = fmaf(x[0], c1, lv);
+          }
+          mx = fmaxf(mx, xm);  // (-inf * 0 where a group has no scale: NaN, dropped)
+        }
+      }
+      m_run = fmaxf(m_run, mx);
+    }
+    // P of block it - SB has been read, O holds blocks up to it - SB
+    if (it >= Tr::SB && !tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][b]), (it / Tr::SB - 1) & 1, abort_flag, 80)) return;
+    const bool move = m_run > m_ref + 8.f;  // (also from -inf)
+    if (__any_sync(0xffffffffu, move)) {
+      const float f = move ? (m_ref == -INFINITY ? 1.f : fast_exp2(m_ref - m_run)) : 1.f;
+      if (move) m_ref = m_run;
+      l *= f;
+      if (it > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+        const int b1 = (it - 1) % Tr::SB;  // O up to block it - 1
+        if (Tr::SB > 1 && !tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][b1]), ((it - 1) / Tr::SB) & 1, abort_flag, 81)) return;
+        tc5::tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < Tr::HD / 32; ++c) {
+          uint32_t r[32];
+          tc5::tmem_ld32(o_tmem + c * 32, r);
+          tc5::tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * f);
+          tc5::tmem_st32(o_tmem + c * 32, r);
+        }
+        tc5::tmem_wait_st();
+      }
+    }
+    const float m_use = m_ref == -INFINITY ? 0.f : m_ref - 7.f;
+    // ---- P' ----
+#pragma unroll
+    for (int c = 0; c < Tr::BN / 32; ++c) {
+      uint32_t r[32], w[16];
+      if (any_live) {
+        tc5::tmem_ld32(s_tmem + c * 32, r);
+        tc5::tmem_wait_ld();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float c1 = sh->sc[e][0][c * 2 + g] * back, lv = sh->sc[e][1][c * 2 + g], inv = sh->sc[e][2][c * 2 + g];
+          const float d = lv - m_use;
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            float x[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const float s = __uint_as_float(r[g * 16 + k + u]);
+              if (CAP) {
+                const float ex = __expf(2.f * (s * c1));
+                x[u] = cap_l2 * (1.f - __fdividef(2.f, ex + 1.f)) + d;
+              } else {
+                x[u] = fmaf(s, c1, d);
+              }
+              if (edge) {
+                const int j = t0 + c * 32 + g * 16 + k + u;
+                if (j < row_lo || j > row_hi) x[u] = -INFINITY;
+              }
+              x[u] = fast_exp2(x[u]);
+            }
+            sum0 += x[0];
+            sum1 += x[1];
+            w[g * 8 + k / 2] = pack2<__half>(x[0], x[1]);
+          }
+          l = fmaf(sum0 + sum1, inv, l);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) w[k] = 0;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // 8 keys = 16 bytes
+        const int ch = (c & 1) * 4 + k;
+        const uint32_t at = p_smem + (c >> 1) * Tr::P_HALF + ((ch ^ (lane_row & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(w[k * 4]), "r"(w[k * 4 + 1]), "r"(w[k * 4 + 2]), "r"(w[k * 4 + 3])
+                     : "memory");
+      }
+    }
+    tc5::tc_fence_before();
+    tc5::fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) {
+      tc5::mbar_arrive(tc5::smem_addr(&sh->s_free[t][b]));
+      tc5::mbar_arrive(tc5::smem_addr(&sh->p_full[t][b]));
+      tc5::mbar_arrive(tc5::smem_addr(&sh->sc_empty[e]));
+    }
+  }
+  // ---- output ----
+  if (sg.cnt > 0) {
+    const int last = sg.cnt - 1;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][last % Tr::SB]), (last / Tr::SB) & 1, abort_flag, 82)) return;
+    tc5::tc_fence_after();
+  }
+  if (!any_live) return;
+  const bool dead = l == 0.f;  // (a NaN is none)
+  const float f = dead ? 0.f : 1.f / l;
+  const float lse = dead ? -INFINITY : (m_ref - 7.f + log2f(l)) * kLn2;
+  const bool to_partial = p.num_splits > 1;
+  const int64_t lse_idx = (int64_t)sg.bi * p.a.lse_batch_stride + (int64_t)head * p.a.lse_head_stride + sq.q_row0 + i;
+  if (live) {
+    if (to_partial) p.lse_partial[(int64_t)sg.slot * p.lse_elems + lse_idx] = lse;
+    else p.a.lse[lse_idx] = dead ? INFINITY : lse;
+  }
+  T* orow = reinterpret_cast<T*>(p.a.o) + (int64_t)sg.bi * p.a.o_batch_stride + (int64_t)(sq.q_row0 + i) * p.a.o_row_stride +
+            (int64_t)head * p.a.o_head_stride;
+  float* prow = to_partial ? p.o_partial + ((int64_t)sg.slot * p.lse_elems + lse_idx) * p.a.d : nullptr;
+#pragma unroll
+  for (int c = 0; c < Tr::HD / 32; ++c) {
+    uint32_t r[32];
+    if (sg.cnt > 0) {
+      tc5::tmem_ld32(o_tmem + c * 32, r);
+      tc5::tmem_wait_ld();
+    }
+    if (live && !(dead && to_partial)) {
+#pragma unroll
+      for (int k = 0; k < 32; k += 8) {
+        if (c * 32 + k < p.a.d) {
+          float x[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) x[u] = dead ? 0.f : __uint_as_float(r[k + u]) * f;
+          if (to_partial) {
+            *reinterpret_cast<float4*>(prow + c * 32 + k) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(prow + c * 32 + k + 4) = make_float4(x[4], x[5], x[6], x[7]);
+          } else {
+            *reinterpret_cast<uint4*>(orow + c * 32 + k) =
+                make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+          }
+        }
+      }
+    }
+    __syncwarp();  // the next columns are loaded by all lanes together
+  }
+}
+
+template <class Tr, int CODE>
+__global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_constant__ Kv8Params p) {
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  __shared__ Kv8TileShared sh;
+  grid_wait();
+  grid_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const Kv8Mask mask = kv8_mask(p, lane);
+  Kv8Walk<Tr::BM, Tr::BN, 0> walk;
+  Kv8Seg sg;
+  walk.first(p, mask, lane, sg);
+  const Kv8Seq sq = kv8_seq(p, mask, sg.bi, sg.mb, Tr::BM);
+  const int rows = sq.q_len * p.group - sg.mb * Tr::BM;
+  if (rows <= 0) return;
+  const int active = Tr::NSUB == 2 && rows > 128 ? 2 : 1;  // sub-tiles with rows
+  if (tid == 0) {
+    for (int s = 0; s < 4; ++s) {
+      tc5::mbar_init(tc5::smem_addr(&sh.kv_full[s]), Tr::CONV_WARPS);
+      tc5::mbar_init(tc5::smem_addr(&sh.kv_empty[s]), active);
+      tc5::mbar_init(tc5::smem_addr(&sh.sc_full[s]), 1);
+      tc5::mbar_init(tc5::smem_addr(&sh.sc_empty[s]), 4 * active);
+    }
+    for (int t = 0; t < 2; ++t) {
+      tc5::mbar_init(tc5::smem_addr(&sh.q_full[t]), 4);
+      for (int b = 0; b < 2; ++b) {
+        tc5::mbar_init(tc5::smem_addr(&sh.s_full[t][b]), 1);
+        tc5::mbar_init(tc5::smem_addr(&sh.s_free[t][b]), 4);
+        tc5::mbar_init(tc5::smem_addr(&sh.p_full[t][b]), 4);
+        tc5::mbar_init(tc5::smem_addr(&sh.pv_done[t][b]), 1);
+      }
+    }
+    sh.abort_flag = 0;
+    tc5::fence_barrier_init();
+  }
+  if (warp == 0) {
+    tc5::tmem_alloc(tc5::smem_addr(&sh.tmem_base), 512);
+    tc5::tmem_relinquish();
+  }
+  tc5::tc_fence_before();
+  __syncthreads();
+  tc5::tc_fence_after();
+  const uint32_t tmem = sh.tmem_base;
+
+  if (warp < Tr::SOFTMAX_WARPS) {
+    const int t = warp >> 2;
+    if (t < active) {
+      const int row = tid - t * 128;
+      const bool cap = p.a.softcap > 0.f;
+      if (p.a.dtype == FA_BF16) {
+        if (cap) kv8_softmax<Tr, __nv_bfloat16, true>(p, mask, sq, sg, &sh, smem, tmem, t, row);
+        else kv8_softmax<Tr, __nv_bfloat16, false>(p, mask, sq, sg, &sh, smem, tmem, t, row);
+      } else {
+        if (cap) kv8_softmax<Tr, __half, true>(p, mask, sq, sg, &sh, smem, tmem, t, row);
+        else kv8_softmax<Tr, __half, false>(p, mask, sq, sg, &sh, smem, tmem, t, row);
+      }
+    }
+  } else if (warp < Tr::SOFTMAX_WARPS + Tr::CONV_WARPS) {
+    const float s = fabsf(p.a.softmax_scale);
+    if (sg.cnt > 0)
+      kv8_convert<Tr, CODE>(p, sq, sg, &sh, smem + Tr::RING_OFF, p.a.softcap > 0.f ? s / p.a.softcap : s * kLog2e, tid - 32 * Tr::SOFTMAX_WARPS);
+  } else {
+    const int t = warp - Tr::SOFTMAX_WARPS - Tr::CONV_WARPS;
+    if (t < active && sg.cnt > 0) kv8_issue<Tr>(&sh, smem, tmem, t, sg.cnt);
+  }
+
+  __syncwarp();
+  tc5::tc_fence_before();
+  __syncthreads();
+  if (sh.abort_flag) {
+    for (int k = 0; k < 64; ++k) __nanosleep(2000);  // let products in flight end before TMEM goes
+    if (tid == 0 && p.status) atomicExch(p.status, (sh.abort_flag << 16) | ((int)blockIdx.x % 0xffff + 1));
+  }
+  if (warp == 0) {
+    tc5::tc_fence_after();
+    tc5::tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace fa

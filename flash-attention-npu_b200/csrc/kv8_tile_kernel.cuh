@@ -11,6 +11,7 @@
 //        4                           converters: codes -> fp16 tiles in the swizzled operand layout; global loads of a tile in flight
 //                                    while the one before is turned
 //        1 per sub-tile              MMA issue
+//        1                           scout: pages and scales, some blocks ahead (and one or two warps fill up the warpgroup)
 // Head dims up to 128: two sub-tiles, whose softmax and products alternate; S0 S1 O0 O1 fill TMEM.  256 columns: one sub-tile
 // with two buffers of S and P for blocks of 64 keys.
 //
@@ -37,18 +38,24 @@ struct Kv8TileTraits {
   static constexpr int RING = HD == 128 ? 3 : 4;
   static constexpr int Q_OFF = 0, P_OFF = NSUB * Q_BYTES, RING_OFF = P_OFF + NSUB * SB * P_BYTES, TAIL_OFF = RING_OFF + RING * SLOT_BYTES;
   static constexpr int SMEM_BYTES = 1024 + TAIL_OFF;
-  static constexpr int SOFTMAX_WARPS = 4 * NSUB, CONV_WARPS = 4, NTHREADS = 32 * (SOFTMAX_WARPS + CONV_WARPS + NSUB);
-  static constexpr int CPR = HD / 16, CHUNKS = BN * CPR / 128;  // 16-code chunks of a key row; of a converter thread in a tile
+  static constexpr int SOFTMAX_WARPS = 4 * NSUB, CONV_WARPS = 4, NTHREADS = 32 * (SOFTMAX_WARPS + CONV_WARPS + 4);
+  // Registers a thread, by warpgroup (setmaxnreg): shares of what the CTA is launched with (128 and 168 a thread), never more.
+  static constexpr int LAUNCH_REGS = NSUB == 2 ? 120 : 152;  // at least
+  static constexpr int SOFTMAX_REGS = NSUB == 2 ? 160 : 208, CONV_REGS = NSUB == 2 ? 112 : 168, ISSUE_REGS = 40;
+  static_assert(32 * (SOFTMAX_WARPS * SOFTMAX_REGS + CONV_WARPS * CONV_REGS + 4 * ISSUE_REGS) <= NTHREADS * LAUNCH_REGS &&
+                NTHREADS * LAUNCH_REGS <= 65536, "more registers than the CTA was launched with");
+  static constexpr int CHUNKS = BN * HD / 16 / 128;  // 16-code chunks of a converter thread in a tile
   static constexpr int O_COL = 256, O_STEP = 128, S_STEP = NSUB == 2 ? 128 : BN;  // TMEM columns
-  static constexpr int SCR = 4;  // blocks of scales in flight
+  static constexpr int SCR = 6;  // blocks that the scout may be ahead
 };
 
 struct Kv8TileShared {
   uint64_t q_full[2], kv_full[4], kv_empty[4];
   uint64_t s_full[2][2], s_free[2][2];  // [sub-tile][buffer]
   uint64_t p_full[2][2], pv_done[2][2];
-  uint64_t sc_full[4], sc_empty[4];
-  float sc[4][3][8];  // of a block: score factor, log2 of V's scale, its reciprocal, per 16 keys
+  uint64_t sc_full[6], sc_empty[6];
+  float sc[6][3][8];   // of a block: score factor, log2 of V's scale, its reciprocal, per 16 keys
+  int64_t at[6][2][8]; // ... and where K's and V's codes of 16 keys start, from the head's first; -1: zeros
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -64,137 +71,127 @@ struct Kv8Ring {
   }
 };
 
-// ---------------- converters ----------------
-template <class Tr, int CODE>
-__device__ __forceinline__ void kv8_convert(const Kv8Params& p, const Kv8Seq& sq, const Kv8Seg& sg, Kv8TileShared* sh, uint32_t ring_smem,
-                                            float mul, int tid) {
-  constexpr int NC = Tr::CHUNKS, CPR = Tr::CPR;
+// ---------------- scout: where a block's keys are, and its scales ----------------
+// One warp, up to SCR blocks ahead: pages and scales are two dependent loads that the converters need not wait for.
+template <class Tr>
+__device__ __forceinline__ void kv8_scout(const Kv8Params& p, const Kv8Seq& sq, const Kv8Seg& sg, Kv8TileShared* sh, float mul, int lane) {
   volatile int* abort_flag = &sh->abort_flag;
-  const int lane = tid & 31, warp = tid >> 5;
-  const int c16 = tid % CPR, row0 = tid / CPR;  // this thread's chunk column, first row; rows advance by 128 / CPR
-  const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.a.k) + (int64_t)sg.hk * p.a.k_head_stride + c16 * 16;
-  const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.a.v) + (int64_t)sg.hk * p.a.v_head_stride + c16 * 16;
-  const bool col_on = c16 * 16 < p.a.d;
-
-  // lane g: page (or cache row) and row in it of the block's 16-key group g; looked up only where a row sees one of its keys
-  struct Where { int outer, row; };
-  auto locate = [&](int it) {
-    const int t = (sg.lo + it) * Tr::BN + lane * kScaleGranule;
-    Where w{0, -1};
-    if (it < sg.cnt && lane < Tr::GROUPS && t < sq.key_hi && t + kScaleGranule > sq.key_lo) {
-      w.outer = sq.batch_row;
-      w.row = t;
+  const bool is_v = lane >= Tr::GROUPS, on = lane < 2 * Tr::GROUPS;  // lanes 0 .. GROUPS - 1: K of 16-key group `lane`, then V
+  const int grp = lane % Tr::GROUPS;
+  const float* scale = is_v ? p.c.v_scale + sg.hk * p.c.vs_head_stride : p.c.k_scale + sg.hk * p.c.ks_head_stride;
+  const int64_t s_outer = is_v ? p.c.vs_outer_stride : p.c.ks_outer_stride, s_block = is_v ? p.c.vs_block_stride : p.c.ks_block_stride;
+  const int64_t c_outer = is_v ? p.a.v_batch_stride : p.a.k_batch_stride, c_row = is_v ? p.a.v_row_stride : p.a.k_row_stride;
+  for (int it = 0; it < sg.cnt; ++it) {
+    const int e = it % Tr::SCR, t = (sg.lo + it) * Tr::BN + grp * kScaleGranule;
+    int64_t at = -1;  // nothing there: zeros
+    float s = 0.f;
+    if (on && t < sq.key_hi && t + kScaleGranule > sq.key_lo) {  // some row sees a key of the group: its page is a live one
+      int outer = sq.batch_row, row = t;
+      bool there = true;
       if (sq.pages) {
-        const int pg = t / p.a.page_size;
-        w.row = t - pg * p.a.page_size;
-        const int id = __ldg(sq.pages + pg);
-        w.outer = outer_index(p.a, id, p.status);
-        if (id != w.outer) w.row = -1;  // not there: zeros
+        const int pg = t / p.a.page_size, id = __ldg(sq.pages + pg);
+        row = t - pg * p.a.page_size;
+        outer = outer_index(p.a, id, p.status);
+        there = outer == id;
+      }
+      if (there) {
+        at = outer * c_outer + row * c_row;
+        s = __ldg(scale + outer * s_outer + (row / p.c.scale_block) * s_block);
       }
     }
-    return w;
-  };
-  auto fetch = [&](uint4 (&x)[NC], const Where& w, int it, bool is_v) {
-    const int t0 = (sg.lo + it) * Tr::BN;
+    if (it >= Tr::SCR && !tc5::mbar_wait(tc5::smem_addr(&sh->sc_empty[e]), (it / Tr::SCR - 1) & 1, abort_flag, 72)) return;
+    if (on) {
+      sh->at[e][is_v][grp] = at;
+      if (!is_v) {
+        sh->sc[e][0][grp] = s * mul;
+      } else {
+        const float v = usable_scale(s);
+        sh->sc[e][1][grp] = log2f(v);
+        sh->sc[e][2][grp] = 1.f / v;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) tc5::mbar_arrive(tc5::smem_addr(&sh->sc_full[e]));
+  }
+}
+
+// ---------------- converters ----------------
+// A thread turns 16-code chunks of column tid % 4 in every 64-column half, of rows tid / 4 + 32 k: two rows of a quarter warp meet eight
+// different banks.
+template <class Tr, int CODE>
+__device__ __forceinline__ void kv8_convert(const Kv8Params& p, const Kv8Seq& sq, const Kv8Seg& sg, Kv8TileShared* sh, uint32_t ring_smem, int tid) {
+  constexpr int NC = Tr::CHUNKS, ROWS = NC / Tr::HALVES;
+  volatile int* abort_flag = &sh->abort_flag;
+  const int lane = tid & 31, c4 = tid & 3, row0 = tid >> 2, in_grp = row0 % kScaleGranule;
+  const int64_t k_rs = p.a.k_row_stride, v_rs = p.a.v_row_stride;
+  const uint8_t* kb = reinterpret_cast<const uint8_t*>(p.a.k) + (int64_t)sg.hk * p.a.k_head_stride + c4 * 16 + in_grp * k_rs;
+  const uint8_t* vb = reinterpret_cast<const uint8_t*>(p.a.v) + (int64_t)sg.hk * p.a.v_head_stride + c4 * 16 + in_grp * v_rs;
+  const int cols_left = p.a.d - c4 * 16;  // halves h with 64 h < cols_left hold columns of the head
+
+  auto fetch = [&](uint4 (&x)[NC], int it, bool is_v) {
+    const int e = it % Tr::SCR, t0 = (sg.lo + it) * Tr::BN;
     const uint8_t* base = is_v ? vb : kb;
-    const int64_t os = is_v ? p.a.v_batch_stride : p.a.k_batch_stride, rs = is_v ? p.a.v_row_stride : p.a.k_row_stride;
+    const bool whole = t0 >= sq.key_lo && t0 + Tr::BN <= sq.key_hi;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int row = row0 + i * (128 / CPR), g = row / kScaleGranule;
-      const int outer = __shfl_sync(0xffffffffu, w.outer, g), r = __shfl_sync(0xffffffffu, w.row, g);
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (r >= 0 && col_on && t0 + row >= sq.key_lo && t0 + row < sq.key_hi)
-        x[i] = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)outer * os + (int64_t)(r + row % kScaleGranule) * rs));
+    for (int k = 0; k < ROWS; ++k) {
+      const int row = row0 + 32 * k;
+      const int64_t at = sh->at[e][is_v][row / kScaleGranule];
+      const bool on = at >= 0 && (whole || (t0 + row >= sq.key_lo && t0 + row < sq.key_hi));
+#pragma unroll
+      for (int h = 0; h < Tr::HALVES; ++h) {
+        uint4& y = x[k * Tr::HALVES + h];
+        y = make_uint4(0, 0, 0, 0);
+        if (on && h * 64 < cols_left) y = __ldg(reinterpret_cast<const uint4*>(base + at + h * 64));
+      }
     }
   };
-  // scales of a block: lanes 0 .. GROUPS - 1 of warp 0 K's, the next ones V's
-  auto fetch_scale = [&](const Where& w) {
-    const int g = lane % Tr::GROUPS;
-    const int outer = __shfl_sync(0xffffffffu, w.outer, g), r = __shfl_sync(0xffffffffu, w.row, g);
-    if (r < 0 || lane >= 2 * Tr::GROUPS) return 0.f;
-    const int64_t blk = r / p.c.scale_block;
-    return lane < Tr::GROUPS ? __ldg(p.c.k_scale + outer * p.c.ks_outer_stride + blk * p.c.ks_block_stride + sg.hk * p.c.ks_head_stride)
-                             : __ldg(p.c.v_scale + outer * p.c.vs_outer_stride + blk * p.c.vs_block_stride + sg.hk * p.c.vs_head_stride);
-  };
-
   Kv8Ring<Tr::RING> ring;
   auto put = [&](const uint4 (&x)[NC]) {
     uint32_t slot, par;
     ring.next(slot, par);
     if (!tc5::mbar_wait(tc5::smem_addr(&sh->kv_empty[slot]), par ^ 1, abort_flag, 71)) return false;
-    const uint32_t tile = ring_smem + slot * Tr::SLOT_BYTES + (c16 >> 2) * Tr::KV_HALF;
+    const uint32_t tile = ring_smem + slot * Tr::SLOT_BYTES + row0 * 128;
+    const uint32_t lo = ((c4 * 2) ^ (row0 & 7)) << 4, hi = ((c4 * 2 + 1) ^ (row0 & 7)) << 4;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int row = row0 + i * (128 / CPR);
+      const uint32_t at = tile + (i % Tr::HALVES) * Tr::KV_HALF + (i / Tr::HALVES) * (32 * 128);
       uint32_t h[8];
       decode4<CODE>(x[i].x, h[0], h[1]);
       decode4<CODE>(x[i].y, h[2], h[3]);
       decode4<CODE>(x[i].z, h[4], h[5]);
       decode4<CODE>(x[i].w, h[6], h[7]);
-      // lanes of odd halves store their second 8 columns first: the eight lanes of a row then meet eight different banks
-      const bool swap = (c16 >> 2) & 1;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool second = (e == 1) != swap;
-        const uint32_t at = tile + row * 128 + ((((c16 & 3) * 2 + (second ? 1 : 0)) ^ (row & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(second ? h[4] : h[0]), "r"(second ? h[5] : h[1]),
-                     "r"(second ? h[6] : h[2]), "r"(second ? h[7] : h[3])
-                     : "memory");
-      }
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + lo), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at + hi), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
     }
     tc5::fence_proxy_async();  // generic-proxy stores -> visible to the MMA
     __syncwarp();
     if (lane == 0) tc5::mbar_arrive(tc5::smem_addr(&sh->kv_full[slot]));
     return true;
   };
-  auto put_scale = [&](int it, float s) {
-    if (warp != 0) return true;
-    const int e = it % Tr::SCR;
-    if (it >= Tr::SCR && !tc5::mbar_wait(tc5::smem_addr(&sh->sc_empty[e]), (it / Tr::SCR - 1) & 1, abort_flag, 72)) return false;
-    if (lane < Tr::GROUPS) {
-      sh->sc[e][0][lane] = s * mul;
-    } else if (lane < 2 * Tr::GROUPS) {
-      const float v = usable_scale(s);
-      sh->sc[e][1][lane - Tr::GROUPS] = log2f(v);
-      sh->sc[e][2][lane - Tr::GROUPS] = 1.f / v;
-    }
-    __syncwarp();
-    if (lane == 0) tc5::mbar_arrive(tc5::smem_addr(&sh->sc_full[e]));
-    return true;
-  };
 
-  // Tiles in ring order, one ahead in registers; the pages of a block are looked up a block before its K is wanted.
-  struct Tile { bool k; int it; };
+  // tiles in ring order, one ahead in registers
   int kq = 0, vq = 0;
-  Where w0 = locate(0), w1 = locate(1), w2 = locate(2);  // of blocks vq, vq + 1, vq + 2
-  auto load = [&](uint4 (&x)[NC], float& s, Tile& tile) {
-    if (vq == sg.cnt) return false;
+  auto load = [&](uint4 (&x)[NC]) {
     if (kq < sg.cnt && kq <= vq + 1) {
-      const Where w = kq == vq ? w0 : w1;
-      tile = Tile{true, kq};
-      fetch(x, w, kq, false);
-      s = fetch_scale(w);
+      if (!tc5::mbar_wait(tc5::smem_addr(&sh->sc_full[kq % Tr::SCR]), (kq / Tr::SCR) & 1, abort_flag, 70)) return false;
+      fetch(x, kq, false);
       ++kq;
     } else {
-      tile = Tile{false, vq};
-      fetch(x, w0, vq, true);
+      if (vq == sg.cnt) return false;
+      fetch(x, vq, true);
+      __syncwarp();
+      if (lane == 0) tc5::mbar_arrive(tc5::smem_addr(&sh->sc_empty[vq % Tr::SCR]));
       ++vq;
-      w0 = w1;
-      w1 = w2;
-      w2 = locate(vq + 2);
     }
     return true;
   };
-  auto emit = [&](const uint4 (&x)[NC], float s, const Tile& tile) { return (!tile.k || put_scale(tile.it, s)) && put(x); };
   uint4 xa[NC], xb[NC];
-  float sa = 0.f, sb = 0.f;
-  Tile ta{}, tb{};
-  bool more = load(xa, sa, ta);
+  bool more = load(xa);
   while (more) {
-    more = load(xb, sb, tb);
-    if (!emit(xa, sa, ta) || !more) return;
-    more = load(xa, sa, ta);
-    if (!emit(xb, sb, tb)) return;
+    more = load(xb);
+    if (!put(xa) || !more) return;
+    more = load(xa);
+    if (!put(xb)) return;
   }
 }
 
@@ -337,43 +334,51 @@ __device__ __forceinline__ void kv8_softmax(const Kv8Params& p, const Kv8Mask& m
     if (!tc5::mbar_wait(tc5::smem_addr(&sh->sc_full[e]), (it / Tr::SCR) & 1, abort_flag, 78)) return;
     if (!tc5::mbar_wait(tc5::smem_addr(&sh->s_full[t][b]), (it / Tr::SB) & 1, abort_flag, 79)) return;
     tc5::tc_fence_after();
+    // (two copies of the code: compares in the common one cost it three times its instructions)
     const bool edge = t0 < all_lo || t0 + Tr::BN > all_hi;
-    if (any_live) {
-      // ---- maximum ----
+    // columns of chunk c (32 keys) that the row sees
+    auto seen = [&](int c) {
+      const int lo = row_lo - (t0 + c * 32), hi = row_hi - (t0 + c * 32);
+      const uint32_t below = hi < 0 ? 0u : hi >= 31 ? 0xffffffffu : (2u << hi) - 1u;
+      return below & (lo <= 0 ? 0xffffffffu : lo >= 32 ? 0u : 0xffffffffu << lo);
+    };
+    auto capped = [&](float z) { return cap_l2 * (1.f - __fdividef(2.f, __expf(2.f * z) + 1.f)); };  // z: score / cap
+    // ---- maximum ----
+    auto find_max = [&](auto masked) {
       float mx = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < Tr::BN / 32; ++c) {
-        uint32_t r[32];
-        tc5::tmem_ld32(s_tmem + c * 32, r);
+      for (int c2 = 0; c2 < Tr::BN / 64; ++c2) {
+        uint32_t r[2][32];
+        tc5::tmem_ld32(s_tmem + c2 * 64, r[0]);
+        tc5::tmem_ld32(s_tmem + c2 * 64 + 32, r[1]);
         tc5::tmem_wait_ld();
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          float x[16];
+        for (int h = 0; h < 2; ++h) {
+          const int c = c2 * 2 + h;
+          const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            x[k] = __uint_as_float(r[g * 16 + k]);
-            if (edge) {
-              const int j = t0 + c * 32 + g * 16 + k;
-              if (j < row_lo || j > row_hi) x[k] = -INFINITY;
+          for (int g = 0; g < 2; ++g) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int k = g * 16; k < g * 16 + 16; k += 2) {
+              float u = __uint_as_float(r[h][k]), v = __uint_as_float(r[h][k + 1]);
+              if (decltype(masked)::value) {
+                if (!(bits >> k & 1)) u = -INFINITY;
+                if (!(bits >> (k + 1) & 1)) v = -INFINITY;
+              }
+              x = fmaxf(x, fmaxf(u, v));
             }
+            const float c1 = sh->sc[e][0][c * 2 + g] * back, lv = sh->sc[e][1][c * 2 + g];
+            float xm;
+            if (CAP) xm = x == -INFINITY ? -INFINITY : capped(x * c1) + lv;
+            else xm = fmaf(x, c1, lv);
+            mx = fmaxf(mx, xm);  // (-inf * 0 where a group has no scale: NaN, dropped)
           }
-#pragma unroll
-          for (int s = 8; s > 0; s >>= 1)
-#pragma unroll
-            for (int k = 0; k < s; ++k) x[k] = fmaxf(x[k], x[k + s]);
-          const float c1 = sh->sc[e][0][c * 2 + g] * back, lv = sh->sc[e][1][c * 2 + g];
-          float xm;
-          if (CAP) {
-            const float ex = __expf(2.f * (x[0] * c1));
-            xm = x[0] == -INFINITY ? -INFINITY : cap_l2 * (1.f - __fdividef(2.f, ex + 1.f)) + lv;
-          } else {
-            xm = fmaf(x[0], c1, lv);
-          }
-          mx = fmaxf(mx, xm);  // (-inf * 0 where a group has no scale: NaN, dropped)
         }
       }
-      m_run = fmaxf(m_run, mx);
-    }
+      return mx;
+    };
+    if (any_live) m_run = fmaxf(m_run, edge ? find_max(std::true_type()) : find_max(std::false_type()));
     // P of block it - SB has been read, O holds blocks up to it - SB
     if (it >= Tr::SB && !tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][b]), (it / Tr::SB - 1) & 1, abort_flag, 80)) return;
     const bool move = m_run > m_ref + 8.f;  // (also from -inf)
@@ -399,52 +404,55 @@ __device__ __forceinline__ void kv8_softmax(const Kv8Params& p, const Kv8Mask& m
     }
     const float m_use = m_ref == -INFINITY ? 0.f : m_ref - 7.f;
     // ---- P' ----
+    auto make_p = [&](auto masked) {
 #pragma unroll
-    for (int c = 0; c < Tr::BN / 32; ++c) {
-      uint32_t r[32], w[16];
-      if (any_live) {
+      for (int c = 0; c < Tr::BN / 32; ++c) {
+        uint32_t r[32], w[16];
         tc5::tmem_ld32(s_tmem + c * 32, r);
         tc5::tmem_wait_ld();
+        const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const float c1 = sh->sc[e][0][c * 2 + g] * back, lv = sh->sc[e][1][c * 2 + g], inv = sh->sc[e][2][c * 2 + g];
-          const float d = lv - m_use;
-          float sum0 = 0.f, sum1 = 0.f;
+          const float c1 = sh->sc[e][0][c * 2 + g] * back, d = sh->sc[e][1][c * 2 + g] - m_use;
+          const uint64_t c12 = tc5::pack_f32x2(c1, c1), d2 = tc5::pack_f32x2(d, d);
+          uint64_t sum2 = tc5::pack_f32x2(0.f, 0.f);
 #pragma unroll
-          for (int k = 0; k < 16; k += 2) {
-            float x[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const float s = __uint_as_float(r[g * 16 + k + u]);
-              if (CAP) {
-                const float ex = __expf(2.f * (s * c1));
-                x[u] = cap_l2 * (1.f - __fdividef(2.f, ex + 1.f)) + d;
-              } else {
-                x[u] = fmaf(s, c1, d);
-              }
-              if (edge) {
-                const int j = t0 + c * 32 + g * 16 + k + u;
-                if (j < row_lo || j > row_hi) x[u] = -INFINITY;
-              }
-              x[u] = fast_exp2(x[u]);
+          for (int k = g * 16; k < g * 16 + 16; k += 2) {
+            float x0, x1;
+            if (CAP) {
+              x0 = capped(__uint_as_float(r[k]) * c1) + d;
+              x1 = capped(__uint_as_float(r[k + 1]) * c1) + d;
+            } else {
+              tc5::unpack_f32x2(tc5::fma_f32x2(tc5::pack_f32x2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), c12, d2), x0, x1);
             }
-            sum0 += x[0];
-            sum1 += x[1];
-            w[g * 8 + k / 2] = pack2<__half>(x[0], x[1]);
+            if (decltype(masked)::value) {
+              if (!(bits >> k & 1)) x0 = -INFINITY;
+              if (!(bits >> (k + 1) & 1)) x1 = -INFINITY;
+            }
+            x0 = fast_exp2(x0);
+            x1 = fast_exp2(x1);
+            sum2 = tc5::add_f32x2(sum2, tc5::pack_f32x2(x0, x1));
+            w[k / 2] = pack2<__half>(x0, x1);
           }
-          l = fmaf(sum0 + sum1, inv, l);
+          float sum0, sum1;
+          tc5::unpack_f32x2(sum2, sum0, sum1);
+          l = fmaf(sum0 + sum1, sh->sc[e][2][c * 2 + g], l);
         }
-      } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) w[k] = 0;
+        for (int k = 0; k < 4; ++k)  // 8 keys = 16 bytes
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(p_smem + (c >> 1) * Tr::P_HALF + ((((c & 1) * 4 + k) ^ (lane_row & 7)) << 4)),
+                       "r"(w[k * 4]), "r"(w[k * 4 + 1]), "r"(w[k * 4 + 2]), "r"(w[k * 4 + 3])
+                       : "memory");
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {  // 8 keys = 16 bytes
-        const int ch = (c & 1) * 4 + k;
-        const uint32_t at = p_smem + (c >> 1) * Tr::P_HALF + ((ch ^ (lane_row & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(w[k * 4]), "r"(w[k * 4 + 1]), "r"(w[k * 4 + 2]), "r"(w[k * 4 + 3])
-                     : "memory");
-      }
+    };
+    if (!any_live) {
+      if (it < Tr::SB)  // stays
+        for (int c = 0; c < Tr::BN / 64 * 8; ++c)
+          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(p_smem + (c >> 3) * Tr::P_HALF + ((c & 7) << 4)), "r"(0) : "memory");
+    } else if (edge) {
+      make_p(std::true_type());
+    } else {
+      make_p(std::false_type());
     }
     tc5::tc_fence_before();
     tc5::fence_proxy_async();
@@ -522,8 +530,10 @@ __global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_
     for (int s = 0; s < 4; ++s) {
       tc5::mbar_init(tc5::smem_addr(&sh.kv_full[s]), Tr::CONV_WARPS);
       tc5::mbar_init(tc5::smem_addr(&sh.kv_empty[s]), active);
+    }
+    for (int s = 0; s < Tr::SCR; ++s) {
       tc5::mbar_init(tc5::smem_addr(&sh.sc_full[s]), 1);
-      tc5::mbar_init(tc5::smem_addr(&sh.sc_empty[s]), 4 * active);
+      tc5::mbar_init(tc5::smem_addr(&sh.sc_empty[s]), 4 * active + Tr::CONV_WARPS);
     }
     for (int t = 0; t < 2; ++t) {
       tc5::mbar_init(tc5::smem_addr(&sh.q_full[t]), 4);
@@ -547,6 +557,7 @@ __global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_
   const uint32_t tmem = sh.tmem_base;
 
   if (warp < Tr::SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(Tr::SOFTMAX_REGS));
     const int t = warp >> 2;
     if (t < active) {
       const int row = tid - t * 128;
@@ -560,12 +571,15 @@ __global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_
       }
     }
   } else if (warp < Tr::SOFTMAX_WARPS + Tr::CONV_WARPS) {
-    const float s = fabsf(p.a.softmax_scale);
-    if (sg.cnt > 0)
-      kv8_convert<Tr, CODE>(p, sq, sg, &sh, smem + Tr::RING_OFF, p.a.softcap > 0.f ? s / p.a.softcap : s * kLog2e, tid - 32 * Tr::SOFTMAX_WARPS);
+    if (Tr::CONV_REGS < Tr::LAUNCH_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Tr::CONV_REGS));
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(Tr::CONV_REGS));
+    if (sg.cnt > 0) kv8_convert<Tr, CODE>(p, sq, sg, &sh, smem + Tr::RING_OFF, tid - 32 * Tr::SOFTMAX_WARPS);
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Tr::ISSUE_REGS));
     const int t = warp - Tr::SOFTMAX_WARPS - Tr::CONV_WARPS;
-    if (t < active && sg.cnt > 0) kv8_issue<Tr>(&sh, smem, tmem, t, sg.cnt);
+    const float s = fabsf(p.a.softmax_scale);
+    if (t == 2) kv8_scout<Tr>(p, sq, sg, &sh, p.a.softcap > 0.f ? s / p.a.softcap : s * kLog2e, lane);
+    else if (t < active && sg.cnt > 0) kv8_issue<Tr>(&sh, smem, tmem, t, sg.cnt);
   }
 
   __syncwarp();

@@ -12,11 +12,16 @@
 //                                    while the one before is turned
 //        1 per sub-tile              MMA issue
 //        1                           scout: pages and scales, some blocks ahead (and one or two warps fill up the warpgroup)
-// Head dims up to 128: two sub-tiles, whose softmax and products alternate; S0 S1 O0 O1 fill TMEM.  256 columns: one sub-tile
-// with two buffers of S and P for blocks of 64 keys.
+// Blocks of 64 keys, two S buffers per sub-tile: S of block j + 1 is there when the softmax of block j ends, so its threads wait for no
+// product.  A thread keeps its 64 scores in registers, and P' goes back into the columns it read, as the TMEM operand of P.V: no
+// shared-memory traffic and no proxy fence for P.  S of block j + 2 lands on P of block j; the same thread issues both products, in
+// this order.  TMEM: per sub-tile S 2 x 64, O 128 columns; one sub-tile with 256 columns of O for head dims above 128.
+// (Before, 128 keys at a time, P through shared memory, S read twice from TMEM: 636 us for four chunks of 301 - 2048 tokens against
+// 1777 - 8192 keys, 32 / 8 heads, of which a third was waiting for products and fences.)
 //
 // Bound: per 128 keys and 256 rows of head dim 128 the products take 2048 cycles of an SM's tensor pipe, the exponentials 2048 of its
-// special-function unit, turning the codes about 1000 of its 8192 issue slots.  TMA cannot convert, so the codes pass through registers.
+// special-function unit, 320 KB through shared memory 2560, turning the codes about 1000 of 8192 issue slots.  TMA cannot convert,
+// so the codes pass through registers.
 #pragma once
 
 #include <type_traits>
@@ -28,34 +33,27 @@ namespace fa {
 template <int HD_>
 struct Kv8TileTraits {
   static constexpr int HD = HD_;
-  static constexpr int NSUB = HD <= 128 ? 2 : 1, SB = 3 - NSUB;  // sub-tiles; S / P buffers of each
-  static constexpr int BM = 128 * NSUB, BN = HD <= 128 ? 128 : 64;
+  static constexpr int NSUB = HD <= 128 ? 2 : 1;  // sub-tiles
+  static constexpr int BM = 128 * NSUB, BN = 64;
   static constexpr int GROUPS = BN / kScaleGranule;
   static constexpr int HALVES = HD / 64;                 // 64-column halves of Q, K, V
   static constexpr int KV_HALF = BN * 128, SLOT_BYTES = HALVES * KV_HALF;
   static constexpr int Q_HALF = 128 * 128, Q_BYTES = HALVES * Q_HALF;  // per sub-tile
-  static constexpr int P_HALF = 128 * 128, P_BYTES = BN / 64 * P_HALF; // per sub-tile and buffer
-  static constexpr int RING = HD == 128 ? 3 : 4;
-  static constexpr int Q_OFF = 0, P_OFF = NSUB * Q_BYTES, RING_OFF = P_OFF + NSUB * SB * P_BYTES, TAIL_OFF = RING_OFF + RING * SLOT_BYTES;
-  static constexpr int SMEM_BYTES = 1024 + TAIL_OFF;
+  static constexpr int RING = HD <= 128 ? 8 : 4;
+  static constexpr int RING_OFF = NSUB * Q_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + RING_OFF + RING * SLOT_BYTES;
   static constexpr int SOFTMAX_WARPS = 4 * NSUB, CONV_WARPS = 4, NTHREADS = 32 * (SOFTMAX_WARPS + CONV_WARPS + 4);
-  // Registers a thread, by warpgroup (setmaxnreg): shares of what the CTA is launched with (128 and 168 a thread), never more.
-  static constexpr int LAUNCH_REGS = NSUB == 2 ? 120 : 152;  // at least
-  static constexpr int SOFTMAX_REGS = NSUB == 2 ? 160 : 208, CONV_REGS = NSUB == 2 ? 112 : 168, ISSUE_REGS = 40;
-  static_assert(32 * (SOFTMAX_WARPS * SOFTMAX_REGS + CONV_WARPS * CONV_REGS + 4 * ISSUE_REGS) <= NTHREADS * LAUNCH_REGS &&
-                NTHREADS * LAUNCH_REGS <= 65536, "more registers than the CTA was launched with");
   static constexpr int CHUNKS = BN * HD / 16 / 128;  // 16-code chunks of a converter thread in a tile
-  static constexpr int O_COL = 256, O_STEP = 128, S_STEP = NSUB == 2 ? 128 : BN;  // TMEM columns
-  static constexpr int SCR = 6;  // blocks that the scout may be ahead
+  static constexpr int O_COL = 256, SUB_STEP = 128;  // TMEM: S of sub-tile t at t * SUB_STEP + buffer * BN, O at O_COL + t * SUB_STEP
+  static constexpr int SCR = 8;  // blocks that the scout may be ahead
 };
 
 struct Kv8TileShared {
-  uint64_t q_full[2], kv_full[4], kv_empty[4];
-  uint64_t s_full[2][2], s_free[2][2];  // [sub-tile][buffer]
-  uint64_t p_full[2][2], pv_done[2][2];
-  uint64_t sc_full[6], sc_empty[6];
-  float sc[6][3][8];   // of a block: score factor, log2 of V's scale, its reciprocal, per 16 keys
-  int64_t at[6][2][8]; // ... and where K's and V's codes of 16 keys start, from the head's first; -1: zeros
+  uint64_t q_full[2], kv_full[8], kv_empty[8];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2][2];  // [sub-tile][buffer]
+  uint64_t sc_full[8], sc_empty[8];
+  float sc[8][3][4];    // of a block: score factor, log2 of V's scale, its reciprocal, per 16 keys
+  int64_t at[8][2][4];  // ... and where K's and V's codes of 16 keys start, from the head's first; -1: zeros
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -200,32 +198,30 @@ template <class Tr>
 __device__ __forceinline__ void kv8_issue(Kv8TileShared* sh, uint32_t smem, uint32_t tmem, int t, int cnt) {
   volatile int* abort_flag = &sh->abort_flag;
   constexpr uint32_t idesc_qk = tc5::make_idesc(0, 128, Tr::BN, 0), idesc_pv = tc5::make_idesc(0, 128, Tr::HD, 1);
-  const uint64_t q_desc = tc5::make_smem_desc(smem + Tr::Q_OFF + t * Tr::Q_BYTES, 16, 1024);
-  const uint64_t p_desc0 = tc5::make_smem_desc(smem + Tr::P_OFF + t * Tr::SB * Tr::P_BYTES, 16, 1024);
+  const uint64_t q_desc = tc5::make_smem_desc(smem + t * Tr::Q_BYTES, 16, 1024);
   const uint64_t k_desc0 = tc5::make_smem_desc(smem + Tr::RING_OFF, 16, 1024);            // K-major
   const uint64_t v_desc0 = tc5::make_smem_desc(smem + Tr::RING_OFF, Tr::KV_HALF, 1024);   // N-contiguous
   constexpr uint64_t kSlot = Tr::SLOT_BYTES >> 4;
   // 16 columns per k-step = 32 bytes inside the 128-byte swizzle span
   auto off = [](int ks, int half) { return (uint64_t)(((ks >> 2) * half + (ks & 3) * 32) >> 4); };
-  const uint32_t o_tmem = tmem + Tr::O_COL + t * Tr::O_STEP;
+  const uint32_t s_tmem0 = tmem + t * Tr::SUB_STEP, o_tmem = tmem + Tr::O_COL + t * Tr::SUB_STEP;
   Kv8Ring<Tr::RING> ring;
   if (!tc5::mbar_wait(tc5::smem_addr(&sh->q_full[t]), 0, abort_flag, 73)) return;
   // a ring slot is free when the products of every sub-tile that has rows have read it
   auto release = [&](uint32_t slot) { tc5::mma_commit(tc5::smem_addr(&sh->kv_empty[slot])); };
+  // The buffer's last P has been read by the product of this thread in front of this one, its scores before that P was written.
   auto qk = [&](int it) {
     uint32_t slot, par;
     ring.next(slot, par);
-    const int b = it % Tr::SB;
     if (!tc5::mbar_wait(tc5::smem_addr(&sh->kv_full[slot]), par, abort_flag, 74)) return false;
-    if (it >= Tr::SB && !tc5::mbar_wait(tc5::smem_addr(&sh->s_free[t][b]), (it / Tr::SB - 1) & 1, abort_flag, 75)) return false;
     tc5::tc_fence_after();
     const uint64_t k_desc = k_desc0 + slot * kSlot;
-    const uint32_t s_tmem = tmem + (Tr::NSUB == 2 ? t : b) * Tr::S_STEP;
+    const uint32_t s_tmem = s_tmem0 + (it & 1) * Tr::BN;
     if (tc5::elect_one()) {
       tc5::mma_ss_c<false>(s_tmem, q_desc, k_desc, idesc_qk);
 #pragma unroll
       for (int ks = 1; ks < Tr::HD / 16; ++ks) tc5::mma_ss_c<true>(s_tmem, q_desc + off(ks, Tr::Q_HALF), k_desc + off(ks, Tr::KV_HALF), idesc_qk);
-      tc5::mma_commit(tc5::smem_addr(&sh->s_full[t][b]));
+      tc5::mma_commit(tc5::smem_addr(&sh->s_full[t][it & 1]));
       release(slot);
     }
     __syncwarp();
@@ -234,28 +230,25 @@ __device__ __forceinline__ void kv8_issue(Kv8TileShared* sh, uint32_t smem, uint
   auto pv = [&](int it) {
     uint32_t slot, par;
     ring.next(slot, par);
-    const int b = it % Tr::SB;
     if (!tc5::mbar_wait(tc5::smem_addr(&sh->kv_full[slot]), par, abort_flag, 76)) return false;
-    if (!tc5::mbar_wait(tc5::smem_addr(&sh->p_full[t][b]), (it / Tr::SB) & 1, abort_flag, 77)) return false;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->p_full[t][it & 1]), (it >> 1) & 1, abort_flag, 77)) return false;
     tc5::tc_fence_after();
-    const uint64_t v_desc = v_desc0 + slot * kSlot, p_desc = p_desc0 + b * (uint64_t)(Tr::P_BYTES >> 4);
+    const uint64_t v_desc = v_desc0 + slot * kSlot;
+    const uint32_t p_tmem = s_tmem0 + (it & 1) * Tr::BN;
     if (tc5::elect_one()) {
-      if (it == 0) tc5::mma_ss_c<false>(o_tmem, p_desc, v_desc, idesc_pv);
-      else tc5::mma_ss_c<true>(o_tmem, p_desc, v_desc, idesc_pv);
+      if (it == 0) tc5::mma_ts_c<false>(o_tmem, p_tmem, v_desc, idesc_pv);
+      else tc5::mma_ts_c<true>(o_tmem, p_tmem, v_desc, idesc_pv);
 #pragma unroll
-      for (int ks = 1; ks < Tr::BN / 16; ++ks)
-        tc5::mma_ss_c<true>(o_tmem, p_desc + off(ks, Tr::P_HALF), v_desc + (uint64_t)(ks * (2048 >> 4)), idesc_pv);
-      tc5::mma_commit(tc5::smem_addr(&sh->pv_done[t][b]));
+      for (int ks = 1; ks < Tr::BN / 16; ++ks) tc5::mma_ts_c<true>(o_tmem, p_tmem + ks * 8, v_desc + (uint64_t)(ks * (2048 >> 4)), idesc_pv);
+      tc5::mma_commit(tc5::smem_addr(&sh->pv_done[t][it & 1]));
       release(slot);
     }
     __syncwarp();
     return true;
   };
-  if (!qk(0)) return;
-  for (int it = 0; it < cnt; ++it) {
-    if (it + 1 < cnt && !qk(it + 1)) return;
-    if (!pv(it)) return;
-  }
+  if (!qk(0) || (cnt > 1 && !qk(1))) return;
+  for (int it = 0; it < cnt; ++it)
+    if (!pv(it) || (it + 2 < cnt && !qk(it + 2))) return;
 }
 
 // ---------------- softmax, one thread per row ----------------
@@ -270,7 +263,7 @@ __device__ __forceinline__ void kv8_softmax(const Kv8Params& p, const Kv8Mask& m
   // ---- Q: fp16, negated for a negative scale (scores then grow with the products), bf16 rows brought into fp16's range ----
   float back = 1.f;
   {
-    const uint32_t q_smem = smem + Tr::Q_OFF + t * Tr::Q_BYTES + lane_row * 128;
+    const uint32_t q_smem = smem + t * Tr::Q_BYTES + lane_row * 128;
     const T* qrow = reinterpret_cast<const T*>(p.a.q) + (int64_t)sg.bi * p.a.q_batch_stride + (int64_t)(sq.q_row0 + i) * p.a.q_row_stride +
                     (int64_t)head * p.a.q_head_stride;
     const bool rot = mask.causal || mask.local;
@@ -324,141 +317,112 @@ __device__ __forceinline__ void kv8_softmax(const Kv8Params& p, const Kv8Mask& m
   const bool any_live = __any_sync(0xffffffffu, live);
   const float cap_l2 = p.a.softcap * kLog2e;
   const uint32_t lane_base = (uint32_t)warp << 21;  // 32 TMEM lanes a warp
-  const uint32_t o_tmem = tmem + Tr::O_COL + t * Tr::O_STEP + lane_base;
+  const uint32_t o_tmem = tmem + Tr::O_COL + t * Tr::SUB_STEP + lane_base;
   float m_ref = -INFINITY, m_run = -INFINITY, l = 0.f;
+  auto capped = [&](float z) { return cap_l2 * (1.f - __fdividef(2.f, __expf(2.f * z) + 1.f)); };  // z: score / cap
 
   for (int it = 0; it < sg.cnt; ++it) {
-    const int b = it % Tr::SB, e = it % Tr::SCR, t0 = (sg.lo + it) * Tr::BN;
-    const uint32_t s_tmem = tmem + (Tr::NSUB == 2 ? t : b) * Tr::S_STEP + lane_base;
-    const uint32_t p_smem = smem + Tr::P_OFF + (t * Tr::SB + b) * Tr::P_BYTES + lane_row * 128;
+    const int b = it & 1, e = it % Tr::SCR, t0 = (sg.lo + it) * Tr::BN;
+    const uint32_t s_tmem = tmem + t * Tr::SUB_STEP + b * Tr::BN + lane_base;
     if (!tc5::mbar_wait(tc5::smem_addr(&sh->sc_full[e]), (it / Tr::SCR) & 1, abort_flag, 78)) return;
-    if (!tc5::mbar_wait(tc5::smem_addr(&sh->s_full[t][b]), (it / Tr::SB) & 1, abort_flag, 79)) return;
+    // (over when S of this block is there; seen so that no phase of the barrier is missed)
+    if (it >= 2 && !tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][b]), ((it >> 1) - 1) & 1, abort_flag, 80)) return;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->s_full[t][b]), (it >> 1) & 1, abort_flag, 79)) return;
     tc5::tc_fence_after();
-    // (two copies of the code: compares in the common one cost it three times its instructions)
-    const bool edge = t0 < all_lo || t0 + Tr::BN > all_hi;
-    // columns of chunk c (32 keys) that the row sees
-    auto seen = [&](int c) {
-      const int lo = row_lo - (t0 + c * 32), hi = row_hi - (t0 + c * 32);
-      const uint32_t below = hi < 0 ? 0u : hi >= 31 ? 0xffffffffu : (2u << hi) - 1u;
-      return below & (lo <= 0 ? 0xffffffffu : lo >= 32 ? 0u : 0xffffffffu << lo);
-    };
-    auto capped = [&](float z) { return cap_l2 * (1.f - __fdividef(2.f, __expf(2.f * z) + 1.f)); };  // z: score / cap
-    // ---- maximum ----
-    auto find_max = [&](auto masked) {
-      float mx = -INFINITY;
+    if (any_live) {  // (rows of the products do not mix: what a warp without rows leaves in P is its own)
+      uint32_t r[2][32];
+      tc5::tmem_ld32(s_tmem, r[0]);
+      tc5::tmem_ld32(s_tmem + 32, r[1]);
+      float c1[4], lv[4];
 #pragma unroll
-      for (int c2 = 0; c2 < Tr::BN / 64; ++c2) {
-        uint32_t r[2][32];
-        tc5::tmem_ld32(s_tmem + c2 * 64, r[0]);
-        tc5::tmem_ld32(s_tmem + c2 * 64 + 32, r[1]);
-        tc5::tmem_wait_ld();
+      for (int g = 0; g < 4; ++g) {
+        c1[g] = sh->sc[e][0][g] * back;
+        lv[g] = sh->sc[e][1][g];
+      }
+      tc5::tmem_wait_ld();
+      const bool edge = t0 < all_lo || t0 + Tr::BN > all_hi;
+      if (edge) {  // some row does not see all: its other scores become -inf, where no bit is set
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int c = c2 * 2 + h;
-          const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
+        for (int c = 0; c < 2; ++c) {
+          const int lo = row_lo - (t0 + c * 32), hi = row_hi - (t0 + c * 32);
+          const uint32_t below = hi < 0 ? 0u : hi >= 31 ? 0xffffffffu : (2u << hi) - 1u;
+          const uint32_t bits = below & (lo <= 0 ? 0xffffffffu : lo >= 32 ? 0u : 0xffffffffu << lo);
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float x = -INFINITY;
+          for (int k = 0; k < 32; ++k)
+            if (!(bits >> k & 1)) r[c][k] = 0xff800000u;
+        }
+      }
+      // ---- maximum ----
 #pragma unroll
-            for (int k = g * 16; k < g * 16 + 16; k += 2) {
-              float u = __uint_as_float(r[h][k]), v = __uint_as_float(r[h][k + 1]);
-              if (decltype(masked)::value) {
-                if (!(bits >> k & 1)) u = -INFINITY;
-                if (!(bits >> (k + 1) & 1)) v = -INFINITY;
-              }
-              x = fmaxf(x, fmaxf(u, v));
-            }
-            const float c1 = sh->sc[e][0][c * 2 + g] * back, lv = sh->sc[e][1][c * 2 + g];
-            float xm;
-            if (CAP) xm = x == -INFINITY ? -INFINITY : capped(x * c1) + lv;
-            else xm = fmaf(x, c1, lv);
-            mx = fmaxf(mx, xm);  // (-inf * 0 where a group has no scale: NaN, dropped)
+      for (int g = 0; g < 4; ++g) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int k = (g & 1) * 16; k < (g & 1) * 16 + 16; k += 2)
+          x = fmaxf(x, fmaxf(__uint_as_float(r[g >> 1][k]), __uint_as_float(r[g >> 1][k + 1])));
+        // a group without a key: -inf, whatever its factors
+        const float xm = x == -INFINITY ? -INFINITY : CAP ? capped(x * c1[g]) + lv[g] : fmaf(x, c1[g], lv[g]);
+        m_run = fmaxf(m_run, xm);
+      }
+      const bool move = m_run > m_ref + 8.f;  // (also from -inf)
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = move ? (m_ref == -INFINITY ? 1.f : fast_exp2(m_ref - m_run)) : 1.f;
+        if (move) m_ref = m_run;
+        l *= f;
+        if (it > 0 && __any_sync(0xffffffffu, f != 1.f)) {  // O up to block it - 1
+          if (!tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][b ^ 1]), ((it - 1) >> 1) & 1, abort_flag, 81)) return;
+          tc5::tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < Tr::HD / 16; ++c) {
+            uint32_t o[16];
+            tc5::tmem_ld16(o_tmem + c * 16, o);
+            tc5::tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tc5::tmem_st16(o_tmem + c * 16, o);
           }
         }
       }
-      return mx;
-    };
-    if (any_live) m_run = fmaxf(m_run, edge ? find_max(std::true_type()) : find_max(std::false_type()));
-    // P of block it - SB has been read, O holds blocks up to it - SB
-    if (it >= Tr::SB && !tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][b]), (it / Tr::SB - 1) & 1, abort_flag, 80)) return;
-    const bool move = m_run > m_ref + 8.f;  // (also from -inf)
-    if (__any_sync(0xffffffffu, move)) {
-      const float f = move ? (m_ref == -INFINITY ? 1.f : fast_exp2(m_ref - m_run)) : 1.f;
-      if (move) m_ref = m_run;
-      l *= f;
-      if (it > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-        const int b1 = (it - 1) % Tr::SB;  // O up to block it - 1
-        if (Tr::SB > 1 && !tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][b1]), ((it - 1) / Tr::SB) & 1, abort_flag, 81)) return;
-        tc5::tc_fence_after();
+      // ---- P' ----
+      const float m_use = m_ref == -INFINITY ? 0.f : m_ref - 7.f;
+      uint32_t w[32];
+      auto make_p = [&](auto masked) {
 #pragma unroll
-        for (int c = 0; c < Tr::HD / 32; ++c) {
-          uint32_t r[32];
-          tc5::tmem_ld32(o_tmem + c * 32, r);
-          tc5::tmem_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * f);
-          tc5::tmem_st32(o_tmem + c * 32, r);
-        }
-        tc5::tmem_wait_st();
-      }
-    }
-    const float m_use = m_ref == -INFINITY ? 0.f : m_ref - 7.f;
-    // ---- P' ----
-    auto make_p = [&](auto masked) {
-#pragma unroll
-      for (int c = 0; c < Tr::BN / 32; ++c) {
-        uint32_t r[32], w[16];
-        tc5::tmem_ld32(s_tmem + c * 32, r);
-        tc5::tmem_wait_ld();
-        const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float c1 = sh->sc[e][0][c * 2 + g] * back, d = sh->sc[e][1][c * 2 + g] - m_use;
-          const uint64_t c12 = tc5::pack_f32x2(c1, c1), d2 = tc5::pack_f32x2(d, d);
+        for (int g = 0; g < 4; ++g) {
+          const float d = lv[g] - m_use;
+          const uint64_t c12 = tc5::pack_f32x2(c1[g], c1[g]), d2 = tc5::pack_f32x2(d, d);
           uint64_t sum2 = tc5::pack_f32x2(0.f, 0.f);
 #pragma unroll
-          for (int k = g * 16; k < g * 16 + 16; k += 2) {
+          for (int k = (g & 1) * 16; k < (g & 1) * 16 + 16; k += 2) {
+            const float s0 = __uint_as_float(r[g >> 1][k]), s1 = __uint_as_float(r[g >> 1][k + 1]);
             float x0, x1;
             if (CAP) {
-              x0 = capped(__uint_as_float(r[k]) * c1) + d;
-              x1 = capped(__uint_as_float(r[k + 1]) * c1) + d;
+              x0 = capped(s0 * c1[g]) + d;
+              x1 = capped(s1 * c1[g]) + d;
             } else {
-              tc5::unpack_f32x2(tc5::fma_f32x2(tc5::pack_f32x2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), c12, d2), x0, x1);
+              tc5::unpack_f32x2(tc5::fma_f32x2(tc5::pack_f32x2(s0, s1), c12, d2), x0, x1);
             }
-            if (decltype(masked)::value) {
-              if (!(bits >> k & 1)) x0 = -INFINITY;
-              if (!(bits >> (k + 1) & 1)) x1 = -INFINITY;
+            if (decltype(masked)::value) {  // hidden is hidden, whatever the factors (-cap, or NaN of -inf * 0)
+              x0 = s0 == -INFINITY ? s0 : x0;
+              x1 = s1 == -INFINITY ? s1 : x1;
             }
             x0 = fast_exp2(x0);
             x1 = fast_exp2(x1);
             sum2 = tc5::add_f32x2(sum2, tc5::pack_f32x2(x0, x1));
-            w[k / 2] = pack2<__half>(x0, x1);
+            w[g * 8 + (k & 15) / 2] = pack2<__half>(x0, x1);
           }
           float sum0, sum1;
           tc5::unpack_f32x2(sum2, sum0, sum1);
-          l = fmaf(sum0 + sum1, sh->sc[e][2][c * 2 + g], l);
+          l = fmaf(sum0 + sum1, sh->sc[e][2][g], l);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // 8 keys = 16 bytes
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(p_smem + (c >> 1) * Tr::P_HALF + ((((c & 1) * 4 + k) ^ (lane_row & 7)) << 4)),
-                       "r"(w[k * 4]), "r"(w[k * 4 + 1]), "r"(w[k * 4 + 2]), "r"(w[k * 4 + 3])
-                       : "memory");
-      }
-    };
-    if (!any_live) {
-      if (it < Tr::SB)  // stays
-        for (int c = 0; c < Tr::BN / 64 * 8; ++c)
-          asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};\n" ::"r"(p_smem + (c >> 3) * Tr::P_HALF + ((c & 7) << 4)), "r"(0) : "memory");
-    } else if (edge) {
-      make_p(std::true_type());
-    } else {
-      make_p(std::false_type());
+      };
+      if (edge) make_p(std::true_type());
+      else make_p(std::false_type());
+      tc5::tmem_st32(s_tmem, w);
+      tc5::tmem_wait_st();  // (and O's)
     }
     tc5::tc_fence_before();
-    tc5::fence_proxy_async();
     __syncwarp();
     if (lane == 0) {
-      tc5::mbar_arrive(tc5::smem_addr(&sh->s_free[t][b]));
       tc5::mbar_arrive(tc5::smem_addr(&sh->p_full[t][b]));
       tc5::mbar_arrive(tc5::smem_addr(&sh->sc_empty[e]));
     }
@@ -466,7 +430,7 @@ __device__ __forceinline__ void kv8_softmax(const Kv8Params& p, const Kv8Mask& m
   // ---- output ----
   if (sg.cnt > 0) {
     const int last = sg.cnt - 1;
-    if (!tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][last % Tr::SB]), (last / Tr::SB) & 1, abort_flag, 82)) return;
+    if (!tc5::mbar_wait(tc5::smem_addr(&sh->pv_done[t][last & 1]), (last >> 1) & 1, abort_flag, 82)) return;
     tc5::tc_fence_after();
   }
   if (!any_live) return;
@@ -527,7 +491,7 @@ __global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_
   if (rows <= 0) return;
   const int active = Tr::NSUB == 2 && rows > 128 ? 2 : 1;  // sub-tiles with rows
   if (tid == 0) {
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < Tr::RING; ++s) {
       tc5::mbar_init(tc5::smem_addr(&sh.kv_full[s]), Tr::CONV_WARPS);
       tc5::mbar_init(tc5::smem_addr(&sh.kv_empty[s]), active);
     }
@@ -539,7 +503,6 @@ __global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_
       tc5::mbar_init(tc5::smem_addr(&sh.q_full[t]), 4);
       for (int b = 0; b < 2; ++b) {
         tc5::mbar_init(tc5::smem_addr(&sh.s_full[t][b]), 1);
-        tc5::mbar_init(tc5::smem_addr(&sh.s_free[t][b]), 4);
         tc5::mbar_init(tc5::smem_addr(&sh.p_full[t][b]), 4);
         tc5::mbar_init(tc5::smem_addr(&sh.pv_done[t][b]), 1);
       }
@@ -557,7 +520,6 @@ __global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_
   const uint32_t tmem = sh.tmem_base;
 
   if (warp < Tr::SOFTMAX_WARPS) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(Tr::SOFTMAX_REGS));
     const int t = warp >> 2;
     if (t < active) {
       const int row = tid - t * 128;
@@ -571,11 +533,8 @@ __global__ void __launch_bounds__(Tr::NTHREADS, 1) kv8_tile_kernel(const __grid_
       }
     }
   } else if (warp < Tr::SOFTMAX_WARPS + Tr::CONV_WARPS) {
-    if (Tr::CONV_REGS < Tr::LAUNCH_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Tr::CONV_REGS));
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(Tr::CONV_REGS));
     if (sg.cnt > 0) kv8_convert<Tr, CODE>(p, sq, sg, &sh, smem + Tr::RING_OFF, tid - 32 * Tr::SOFTMAX_WARPS);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Tr::ISSUE_REGS));
     const int t = warp - Tr::SOFTMAX_WARPS - Tr::CONV_WARPS;
     const float s = fabsf(p.a.softmax_scale);
     if (t == 2) kv8_scout<Tr>(p, sq, sg, &sh, p.a.softcap > 0.f ? s / p.a.softcap : s * kLog2e, lane);

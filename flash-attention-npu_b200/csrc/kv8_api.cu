@@ -39,6 +39,7 @@ struct Kv8Plan {
   Kv8TileInfo tile;
   int hd, grid;
   bool wide, tiled;
+  int subs;
   size_t lse_bytes, workspace_bytes;
 };
 
@@ -110,7 +111,8 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   out->hd = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
   out->wide = rows_max > 16;
   out->tiled = rows_max > 32;
-  out->tile = out->tiled ? kv8_tile_info(out->hd) : kv8_decode_info(out->hd, out->wide);
+  out->subs = rows_max > 128 && out->hd <= 128 ? 2 : 1;
+  out->tile = out->tiled ? kv8_tile_info(out->hd, out->subs) : kv8_decode_info(out->hd, out->wide);
   const Kv8TileInfo& t = out->tile;
   p.m_blocks = std::max(1, ceil_div(rows_max, t.block_m));
   p.box_rows = t.block_n;
@@ -126,9 +128,9 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   int ns = 1;
   if (a.num_splits >= 1) {
     ns = std::min(a.num_splits, max_blocks);
-  } else if (out->tiled) {
+  } else if (p.m_blocks > 1) {
     // as many key ranges as fill the chip, of at least eight blocks each
-    if (units < num_sm) ns = (int)std::max<long long>(1, std::min<long long>(num_sm / units, max_blocks / 8));
+    if (units < slots) ns = (int)std::max<long long>(1, std::min<long long>(slots / units, max_blocks / 8));
   } else if (max_blocks >= 4) {
     p.persistent = 1;
     ns = 4;
@@ -178,7 +180,10 @@ static int run_kv8_fwd(const fa_fwd_params& a_in, const fa_kv8_cache& c, void* w
   }
   cudaError_t e;
   if (P.tiled) {
-    e = P.hd == 64 ? launch_kv8_tile_64(p, P.grid, st) : P.hd == 128 ? launch_kv8_tile_128(p, P.grid, st) : launch_kv8_tile_256(p, P.grid, st);
+    auto* launch = P.hd == 64    ? (P.subs == 1 ? launch_kv8_tile_64_1 : launch_kv8_tile_64_2)
+                   : P.hd == 128 ? (P.subs == 1 ? launch_kv8_tile_128_1 : launch_kv8_tile_128_2)
+                                 : launch_kv8_tile_256_1;
+    e = launch(p, P.grid, st);
   } else {
     CUtensorMap tm_k, tm_v;
     const int64_t rows = a.block_table ? a.page_size : a.seqlen_k, outer = a.kv_outer > 0 ? a.kv_outer : a.b;

@@ -14,11 +14,10 @@ Kv8TileInfo kv8_decode_info(int hd, bool wide) {
   return wide ? info<Kv8Traits<256, 2>>() : info<Kv8Traits<256, 1>>();
 }
 
-template <class Tr>
-static Kv8TileInfo tile_info() { return Kv8TileInfo{Tr::BM, Tr::BN, Tr::NTHREADS, Tr::SMEM_BYTES, 1}; }
-
-Kv8TileInfo kv8_tile_info(int hd) {
-  return hd == 64 ? tile_info<Kv8TileTraits<64>>() : hd == 128 ? tile_info<Kv8TileTraits<128>>() : tile_info<Kv8TileTraits<256>>();
+Kv8TileInfo kv8_tile_info(int hd, int subs) {
+  if (hd == 64) return subs == 1 ? info<Kv8TileTraits<64, 1>>() : info<Kv8TileTraits<64, 2>>();
+  if (hd == 128) return subs == 1 ? info<Kv8TileTraits<128, 1>>() : info<Kv8TileTraits<128, 2>>();
+  return info<Kv8TileTraits<256, 1>>();
 }
 
 }  // namespace fa

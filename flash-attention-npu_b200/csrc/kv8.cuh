@@ -112,10 +112,12 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Params& p, const Kv8Mask& m, 
 
 // ---- the work list of a CTA ----
 // A unit is a row tile of one (sequence, kv head).  One unit (or one of its key splits) per CTA, or resident CTAs with equal
-// shares of all units' key blocks: the units are laid end to end, each as its key blocks (one, fully masked, when it sees no
-// key, so that its rows are written) behind `kOvh` virtual blocks that stand for its fixed cost; CTA c takes virtual blocks
-// [c * quota, (c + 1) * quota).  A unit that CTA boundaries cut leaves one partial per CTA in consecutive slots.  Producer and
-// consumer warps walk the list independently of one another.
+// shares of all units' key blocks: gridDim.x / h_k CTAs a kv head, head fastest, so that the heads of a token, which are neighbours in memory,
+// are read at the same time (8 sequences of 131072 keys, 8 heads of 128 bytes: 402 us with one unit after the other).  A head's units are
+// laid end to end, each as its key blocks (one, fully masked, when it sees no key, so that its rows are written) behind OVH
+// virtual blocks that stand for its fixed cost; CTA c of the head takes virtual blocks [c * quota, (c + 1) * quota).  A unit that
+// CTA boundaries cut leaves one partial per CTA in consecutive slots.  Producer and consumer warps walk the list independently of one
+// another.
 struct Kv8Seg {
   int bi, hk, mb;
   int lo, cnt;          // key blocks [lo, lo + cnt)
@@ -126,7 +128,7 @@ struct Kv8Seg {
 
 template <int BM, int BN, int OVH>
 struct Kv8Walk {
-  int bi, hk, nb_lo, nb_hi, n_b, quota, cur, g1, ustart;
+  int bi, nb_lo, nb_hi, n_b, quota, cur, g1, ustart;
 
   __device__ __forceinline__ static void blocks(const Kv8Params& p, const Kv8Mask& m, int bi, int mb, int& nb_lo, int& nb_hi) {
     const int q_len = kv8_q_len(p, bi), k_len = kv8_k_len(p, bi);
@@ -145,19 +147,16 @@ struct Kv8Walk {
     }
     const int seg_lo = cur - ustart, seg_hi = min(n_b, g1 - ustart);
     const int lo = max(seg_lo - OVH, 0), hi = max(seg_hi - OVH, 0);
-    const int first_cta = (ustart + OVH) / quota;  // the CTA that holds the first real block
+    const int first_cta = (ustart + OVH) / quota;  // the CTA (of this head's) that holds the first real block
     const bool first = lo == 0 && hi > 0;
-    sg = Kv8Seg{bi, hk, 0, nb_lo + lo, hi - lo, (int)blockIdx.x - first_cta,
+    sg = Kv8Seg{bi, (int)blockIdx.x % p.a.h_k, 0, nb_lo + lo, hi - lo, (int)blockIdx.x / p.a.h_k - first_cta,
                 first ? (ustart + n_b - 1) / quota - first_cta + 1 : p.num_splits, nb_hi <= nb_lo, hi > lo ? 1 : 2};
     cur = ustart + seg_hi;
     if (seg_hi == n_b) {
       ustart += n_b;
-      if (++hk == p.a.h_k) {
-        hk = 0;
-        if (++bi < p.a.b) {
-          blocks(p, m, bi, 0, nb_lo, nb_hi);
-          n_b = max(1, nb_hi - nb_lo) + OVH;
-        }
+      if (++bi < p.a.b) {
+        blocks(p, m, bi, 0, nb_lo, nb_hi);
+        n_b = max(1, nb_hi - nb_lo) + OVH;
       }
     }
   }
@@ -165,7 +164,7 @@ struct Kv8Walk {
   // warp-collective: the first segment of this CTA
   __device__ __forceinline__ void first(const Kv8Params& p, const Kv8Mask& m, int lane, Kv8Seg& sg) {
     const int nbat = p.a.b;
-    bi = hk = nb_lo = nb_hi = cur = g1 = ustart = 0;
+    bi = nb_lo = nb_hi = cur = g1 = ustart = 0;
     n_b = quota = 1;
     if (!p.persistent) {  // kv head fastest, then row tile, split, sequence
       int idx = blockIdx.x;
@@ -198,10 +197,10 @@ struct Kv8Walk {
         sm += __shfl_xor_sync(0xffffffffu, sm, o);
       }
       n_max = max(n_max, mx);
-      total += sm * p.a.h_k;
+      total += sm;
     }
-    quota = max(ceil_div(total, (int)gridDim.x), ceil_div(n_max - OVH, p.num_splits - 1));
-    cur = (int)blockIdx.x * quota;
+    quota = max(ceil_div(total, (int)gridDim.x / p.a.h_k), ceil_div(n_max - OVH, p.num_splits - 1));
+    cur = (int)blockIdx.x / p.a.h_k * quota;
     g1 = min(total, cur + quota);
     bi = nbat;
     if (cur < g1) {
@@ -211,7 +210,7 @@ struct Kv8Walk {
           blocks(p, m, b0 + lane, 0, lo, hi);
           n = max(1, hi - lo) + OVH;
         }
-        int incl = n * p.a.h_k;
+        int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int y = __shfl_up_sync(0xffffffffu, incl, o);
@@ -221,7 +220,7 @@ struct Kv8Walk {
         if (hit) {
           const int src = __ffs(hit) - 1;
           bi = b0 + src;
-          ustart += __shfl_sync(0xffffffffu, incl - n * p.a.h_k, src);
+          ustart += __shfl_sync(0xffffffffu, incl - n, src);
           nb_lo = __shfl_sync(0xffffffffu, lo, src);
           nb_hi = __shfl_sync(0xffffffffu, hi, src);
           n_b = __shfl_sync(0xffffffffu, n, src);
@@ -229,8 +228,6 @@ struct Kv8Walk {
           ustart += __shfl_sync(0xffffffffu, incl, 31);
         }
       }
-      hk = (cur - ustart) / n_b;
-      ustart += hk * n_b;
     }
     next(p, m, sg);
   }

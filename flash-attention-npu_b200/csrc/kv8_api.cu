@@ -38,8 +38,8 @@ struct Kv8Plan {
   Kv8Params p;
   Kv8TileInfo tile;
   int hd, grid;
-  bool wide, tiled;
-  int subs;
+  bool tiled;
+  int subs;  // tile kernel: sub-tiles
   size_t lse_bytes, workspace_bytes;
 };
 
@@ -109,10 +109,9 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   // ---- tile and key splits ----
   const int rows_max = a.seqlen_q * p.group;
   out->hd = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
-  out->wide = rows_max > 16;
   out->tiled = rows_max > 32;
   out->subs = rows_max > 128 && out->hd <= 128 ? 2 : 1;
-  out->tile = out->tiled ? kv8_tile_info(out->hd, out->subs) : kv8_decode_info(out->hd, out->wide);
+  out->tile = out->tiled ? kv8_tile_info(out->hd, out->subs) : kv8_decode_info(out->hd, rows_max <= 8 ? 8 : rows_max <= 16 ? 16 : 32);
   const Kv8TileInfo& t = out->tile;
   p.m_blocks = std::max(1, ceil_div(rows_max, t.block_m));
   p.box_rows = t.block_n;
@@ -141,7 +140,7 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
     ns = ceil_div(max_blocks, p.blocks_per_split);
   }
   p.num_splits = ns;
-  out->grid = (int)(p.persistent ? slots : units * ns);
+  out->grid = (int)(p.persistent ? std::max(1LL, slots / a.h_k) * a.h_k : units * ns);
   const bool varlen = a.cu_seqlens_q != nullptr;
   p.lse_elems = varlen ? (int64_t)a.h * a.total_q : (int64_t)a.b * a.h * a.seqlen_q;
   if (varlen ? a.lse_head_stride != a.total_q : (a.lse_head_stride != a.seqlen_q || a.lse_batch_stride != (int64_t)a.h * a.seqlen_q))
@@ -195,7 +194,7 @@ static int run_kv8_fwd(const fa_fwd_params& a_in, const fa_kv8_cache& c, void* w
     auto* launch = P.hd == 64    ? (e4m3 ? launch_kv8_decode_64_e4m3 : launch_kv8_decode_64_int8)
                    : P.hd == 128 ? (e4m3 ? launch_kv8_decode_128_e4m3 : launch_kv8_decode_128_int8)
                                  : (e4m3 ? launch_kv8_decode_256_e4m3 : launch_kv8_decode_256_int8);
-    e = launch(P.wide, p, tm_k, tm_v, P.grid, st);
+    e = launch(P.tile.block_m, p, tm_k, tm_v, P.grid, st);
   }
   if (e != cudaSuccess) return cuda_fail("attention kernel launch", e);
   count_launches(1);

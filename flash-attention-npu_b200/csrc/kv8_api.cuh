@@ -8,10 +8,10 @@ namespace fa {
 struct Kv8TileInfo {
   int block_m, block_n, threads, smem_bytes, resident;
 };
-// Decode kernel: `hd` tile width (64, 128, 256), `wide`: tiles of 32 rows instead of 16.
-Kv8TileInfo kv8_decode_info(int hd, bool wide);
+// Decode kernel: `hd` tile width (64, 128, 256), tiles of 8, 16 or 32 rows.
+Kv8TileInfo kv8_decode_info(int hd, int rows);
 #define FA_KV8_LAUNCHER(NAME_) \
-  cudaError_t NAME_(bool wide, const Kv8Params& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, int grid, cudaStream_t st);
+  cudaError_t NAME_(int rows, const Kv8Params& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, int grid, cudaStream_t st);
 FA_KV8_LAUNCHER(launch_kv8_decode_64_e4m3)
 FA_KV8_LAUNCHER(launch_kv8_decode_64_int8)
 FA_KV8_LAUNCHER(launch_kv8_decode_128_e4m3)

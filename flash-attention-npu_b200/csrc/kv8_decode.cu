@@ -8,11 +8,11 @@ namespace fa {
 template <class Tr>
 static Kv8TileInfo info() { return Kv8TileInfo{Tr::BM, Tr::BN, Tr::NTHREADS, Tr::SMEM_BYTES, Tr::RESIDENT}; }
 
-Kv8TileInfo kv8_decode_info(int hd, bool wide) {
-  if (hd == 64) return wide ? info<Kv8Traits<64, 2>>() : info<Kv8Traits<64, 1>>();
-  if (hd == 128) return wide ? info<Kv8Traits<128, 2>>() : info<Kv8Traits<128, 1>>();
-  return wide ? info<Kv8Traits<256, 2>>() : info<Kv8Traits<256, 1>>();
+template <int HD>
+static Kv8TileInfo decode_info(int rows) {
+  return rows == 8 ? info<Kv8Traits<HD, 1, 1>>() : rows == 16 ? info<Kv8Traits<HD, 1, 2>>() : info<Kv8Traits<HD, 2, 2>>();
 }
+Kv8TileInfo kv8_decode_info(int hd, int rows) { return hd == 64 ? decode_info<64>(rows) : hd == 128 ? decode_info<128>(rows) : decode_info<256>(rows); }
 
 Kv8TileInfo kv8_tile_info(int hd, int subs) {
   if (hd == 64) return subs == 1 ? info<Kv8TileTraits<64, 1>>() : info<Kv8TileTraits<64, 2>>();

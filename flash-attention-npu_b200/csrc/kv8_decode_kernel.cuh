@@ -10,12 +10,15 @@
 // with is largest.  P' is rounded to fp16 (2^-12) for the second product, which is what a 16-bit output can show; the codes
 // are fp16 values, sums and statistics are fp32.
 //
+// Both products are transposed, S^T = K Q^T and O^T = V^T P^T: query rows are the narrow side of mma m16n8k16, so that the eight rows
+// of a usual query group fill it (with rows on the wide side half of every product was padding).  P^T comes out of S^T by a transposition
+// of 8 x 8 tiles within the warp (movmatrix).
 // Fragments straight from the codes.  A contraction may run over its index in any order, and output columns may be numbered in
-// any order, as long as both operands agree: lane (g8, t4) takes LB consecutive bytes of key row g8 as the K elements of its k-steps
-// (four a step), and for V VB consecutive bytes of four key rows as the columns of as many n-tiles, two rows' bytes interleaved
-// by a byte permutation.  So every shared-memory access is a wide one, free of bank conflicts under the TMA swizzle, and each code
-// is turned once: per 16 keys of head dim 128 a warp issues 8 loads, 64 conversions, 16 permutations and 32 mma (64 cycles of an
-// SM's mma.sync rate, against 178 cycles in which HBM delivers the bytes).
+// any order, as long as both operands agree: lane (g8, t4) takes LB consecutive bytes of key rows g8 and g8 + 8 as the K elements of
+// its k-steps (four a step), and for V VB consecutive bytes of four key rows as columns g8 and g8 + 8 of VB / 2 tiles, two
+// rows' bytes interleaved by a byte permutation.  So every shared-memory access is a wide one, free of bank conflicts under the TMA
+// swizzle, and each code is turned once: per 16 keys of head dim 128 and 8 rows a warp issues 8 loads, 64 conversions, 16 permutations
+// and 16 mma (32 cycles of an SM's mma.sync rate, against 178 cycles in which HBM delivers the bytes).
 #pragma once
 
 #include <type_traits>
@@ -24,15 +27,15 @@
 
 namespace fa {
 
-template <int HD_, int WM_>
+template <int HD_, int WM_, int NQ_>
 struct Kv8Traits {
-  static constexpr int HD = HD_, WM = WM_, WN = 4, NCW = WM * WN;
+  static constexpr int HD = HD_, WM = WM_, NQ = NQ_, WN = 4, NCW = WM * WN;  // NQ: 8-row tiles of a warp; WM warps' rows, WN warps' keys
   static_assert(HD == 64 || HD == 128 || HD == 256, "tile widths; a head dim below the width leaves zero columns (TMA fill)");
-  static constexpr int BM = 16 * WM;
+  static constexpr int BM = 8 * NQ * WM;
   static constexpr int BN = HD == 256 ? 64 : 128;
   static constexpr int NTHREADS = 32 * (NCW + 1);
   static constexpr int NW = BN / WN;   // keys of a consumer warp in a stage
-  static constexpr int NT = NW / 8;
+  static constexpr int NG = NW / kScaleGranule;  // 16-key groups of them
   static constexpr int KS = HD / 16;
   static constexpr int ROWB = HD < 128 ? HD : 128;  // bytes of a key row in one TMA box (the swizzle's span)
   static constexpr int HALVES = HD / ROWB;
@@ -41,7 +44,7 @@ struct Kv8Traits {
   static constexpr int HALF_BYTES = BN * ROWB;
   static constexpr int KV_BYTES = HALVES * HALF_BYTES;
   static constexpr int STAGE_BYTES = 2 * KV_BYTES;
-  // 16 rows: two resident CTAs of 96 KiB rings (64 columns: 80 KiB); 32 rows: one CTA with all of it (64 columns: two)
+  // up to 16 rows: two resident CTAs of 96 KiB rings (64 columns: 80 KiB); 32 rows: one CTA with all of it (64 columns: two)
   static constexpr int RESIDENT = WM == 1 || HD == 64 ? 2 : 1;
   static constexpr int ST = HD == 64 ? 5 : WM == 1 ? 3 : 5;
   static constexpr int GROUPS = BN / kScaleGranule;
@@ -55,7 +58,7 @@ struct Kv8Traits {
   static constexpr int BAR_BYTES = 2 * ST * 8;
   // [ring | Q or rows | (m, l) | scales | row factors | barriers], the ring at a 1024-byte aligned base
   static constexpr int SMEM_BYTES = 1024 + PIPE_BYTES + TILE_BYTES + ML_BYTES + SC_BYTES + BM * 4 + BAR_BYTES;
-  static constexpr bool Q_IN_REGS = HD <= 128;
+  static constexpr bool Q_IN_REGS = HD * NQ <= 256;
   static_assert(SMEM_BYTES * RESIDENT <= 227 * 1024 - 2048 * RESIDENT, "shared memory");
 };
 
@@ -68,7 +71,8 @@ __device__ __forceinline__ uint32_t code_addr(uint32_t tile, int row, int ch) {
 __device__ __forceinline__ void lds128(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
-__device__ __forceinline__ void lds64(uint32_t (&r)[4], uint32_t addr) {
+template <int N>
+__device__ __forceinline__ void lds64(uint32_t (&r)[N], uint32_t addr) {
   asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];\n" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
 }
 __device__ __forceinline__ float lds32f(uint32_t addr) {
@@ -135,7 +139,7 @@ __device__ __forceinline__ bool kv8_producer(const Kv8Params& p, const Kv8Seq& s
   return true;
 }
 
-// Q rows -> fp16 fragments in shared memory, [k-step][lane][4 registers], and the factor of each row.
+// Q rows -> fp16 fragments in shared memory, [8-row tile][k-step][lane][2 registers], and the factor of each row.
 template <class Tr, typename T>
 __device__ __forceinline__ void kv8_load_q(const Kv8Params& p, const Kv8Seq& sq, const Kv8Seg& sg, uint32_t q_base, float* factor,
                                            bool rot_per_token, int warp, int lane) {
@@ -171,18 +175,23 @@ __device__ __forceinline__ void kv8_load_q(const Kv8Params& p, const Kv8Seq& sq,
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const int ks = half * (Tr::LB / 4) + (col % Tr::LB) / 4 + st;
-      const uint32_t at = q_base + ((ks * 32 + (row & 7) * 4 + t4) * 4 + ((row >> 3) & 1)) * 4 + (row >> 4) * (Tr::KS * 512);
-      asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(at), "r"(w[2 * st]) : "memory");
-      asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(at + 8), "r"(w[2 * st + 1]) : "memory");
+      const uint32_t at = q_base + (((row >> 3) * Tr::KS + ks) * 32 + (row & 7) * 4 + t4) * 8;
+      asm volatile("st.shared.v2.b32 [%0], {%1,%2};\n" ::"r"(at), "r"(w[2 * st]), "r"(w[2 * st + 1]) : "memory");
     }
   }
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
+  return r;
 }
 
 template <class Tr, int CODE>
 __global__ void __launch_bounds__(Tr::NTHREADS, Tr::RESIDENT)
 kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-  constexpr int NT = Tr::NT, KS = Tr::KS, BN = Tr::BN, BM = Tr::BM, ST = Tr::ST, WN = Tr::WN, NCW = Tr::NCW, NCT = NCW * 32;
-  constexpr int DT = Tr::HD / 8;  // n-tiles of the output
+  constexpr int NG = Tr::NG, NQ = Tr::NQ, KS = Tr::KS, BN = Tr::BN, BM = Tr::BM, ST = Tr::ST, WN = Tr::WN, NCW = Tr::NCW, NCT = NCW * 32;
+  constexpr int DT = Tr::HD / 16;  // 16-column tiles of the output
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_lse[BM];
   __shared__ int s_abort;
@@ -240,7 +249,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
       if (lane == 0) s_seg = sg;
     }
     const int wm = warp / WN, wn = warp % WN;
-    const uint32_t q_frag = q_base + wm * (KS * 512) + lane * 16;
+    const uint32_t q_frag = q_base + wm * (NQ * KS * 256) + lane * 8;
     const bool to_partial = p.persistent || p.num_splits > 1, has_softcap = p.a.softcap > 0.f;
     const float sc_mul = has_softcap ? p.a.softmax_scale / p.a.softcap : p.a.softmax_scale * kLog2e;
     const float cap_l2 = p.a.softcap * kLog2e;
@@ -258,29 +267,37 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
         else kv8_load_q<Tr, __half>(p, sq, sg, q_base, factor, per_token, warp, lane);
         asm volatile("bar.sync 1, %0;\n" ::"n"(NCT));
 
-        float o_acc[DT][4], m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f}, mul[2];
-        int row_lo[2], row_hi[2];
+        // lane (g8, t4): query rows 8 nq + 2 t4 + u (u = 0, 1) of this warp's, keys g8 and g8 + 8 of every 16
+        float o_acc[DT][NQ][4], m_run[NQ][2], l_run[NQ][2], mul[NQ][2];
+        int row_lo[NQ][2], row_hi[NQ][2];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o_acc[dt][e] = 0.f;
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int r = wm * 16 + g8 + 8 * hf, i = (sg.mb * BM + r) / p.group;
-          int lo = 0, hi = sq.k_len - 1;
-          if (mask.causal) hi = min(hi, i + sq.koff);
-          if (mask.local) {
-            hi = min(hi, i + sq.koff + mask.wr);
-            lo = max(0, i + sq.koff - mask.wl);
+            for (int e = 0; e < 4; ++e) o_acc[dt][nq][e] = 0.f;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int r = (wm * NQ + nq) * 8 + 2 * t4 + u, i = (sg.mb * BM + r) / p.group;
+            int lo = 0, hi = sq.k_len - 1;
+            if (mask.causal) hi = min(hi, i + sq.koff);
+            if (mask.local) {
+              hi = min(hi, i + sq.koff + mask.wr);
+              lo = max(0, i + sq.koff - mask.wl);
+            }
+            row_lo[nq][u] = lo;
+            row_hi[nq][u] = r < rows ? hi : -1;
+            mul[nq][u] = factor[r] * sc_mul;
+            m_run[nq][u] = -INFINITY;
+            l_run[nq][u] = 0.f;
           }
-          row_lo[hf] = lo;
-          row_hi[hf] = r < rows ? hi : -1;
-          mul[hf] = factor[r] * sc_mul;
         }
-        uint32_t qf[Tr::Q_IN_REGS ? KS : 1][4];
+        uint32_t qf[Tr::Q_IN_REGS ? KS : 1][NQ][2];
         if (Tr::Q_IN_REGS) {
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) lds128(qf[ks], q_frag + ks * 512);
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) lds64(qf[ks][nq], q_frag + (nq * KS + ks) * 256);
         }
         // every row of the tile sees keys [all_lo, all_hi)
         const int i_first = sg.mb * BM / p.group, i_last = (sg.mb * BM + rows - 1) / p.group;
@@ -299,119 +316,139 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
           const uint32_t sc = scales + stage * (2 * Tr::GROUPS * 4) + (wn * Tr::NW / kScaleGranule) * 4;
           const int t0 = (sg.lo + it) * BN, col0 = t0 + wn * Tr::NW;
 
-          float s_acc[NT][4];
+          // [2 h + u]: key g8 + 8 h, row u.  At least four sums side by side: one product waits 30 cycles for the one before it.
+          constexpr int PARTS = NG * NQ >= 4 ? 1 : 4 / (NG * NQ);
+          float s_part[PARTS][NG][NQ][4], (&s_acc)[NG][NQ][4] = s_part[0];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int pt = 0; pt < PARTS; ++pt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s_acc[nt][e] = 0.f;
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s_part[pt][g][nq][e] = 0.f;
 #pragma unroll
           for (int cj = 0; cj < KS / 4; ++cj) {  // 16 bytes of a key row: four k-steps
             const int ch = Tr::ROWB == 128 ? (cj >> 1) * 8 + 2 * t4 + (cj & 1) : t4;
-            uint32_t a[4][4];
+            uint32_t q2[4][NQ][2];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              if (Tr::Q_IN_REGS) {
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a[s][e] = qf[cj * 4 + s][e];
-              } else {
-                lds128(a[s], q_frag + (cj * 4 + s) * 512);
+              for (int nq = 0; nq < NQ; ++nq) {
+                if (Tr::Q_IN_REGS) {
+                  q2[s][nq][0] = qf[cj * 4 + s][nq][0];
+                  q2[s][nq][1] = qf[cj * 4 + s][nq][1];
+                } else {
+                  lds64(q2[s][nq], q_frag + (nq * KS + cj * 4 + s) * 256);
+                }
               }
-            }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t kw[4];
-              lds128(kw, code_addr<Tr>(k_base, wn * Tr::NW + nt * 8 + g8, ch));
+            for (int g = 0; g < NG; ++g) {
+              uint32_t ka[4], kb[4];
+              lds128(ka, code_addr<Tr>(k_base, wn * Tr::NW + g * 16 + g8, ch));
+              lds128(kb, code_addr<Tr>(k_base, wn * Tr::NW + g * 16 + 8 + g8, ch));
 #pragma unroll
               for (int s = 0; s < 4; ++s) {
-                uint32_t b0, b1;
-                decode4<CODE>(kw[s], b0, b1);
-                mma_16816<__half>(s_acc[nt], a[s], b0, b1);
+                uint32_t a[4];
+                decode4<CODE>(ka[s], a[0], a[2]);
+                decode4<CODE>(kb[s], a[1], a[3]);
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) mma_16816<__half>(s_part[s % PARTS][g][nq], a, q2[s][nq][0], q2[s][nq][1]);
               }
             }
           }
 
+#pragma unroll
+          for (int pt = 1; pt < PARTS; ++pt)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s_acc[g][nq][e] += s_part[pt][g][nq][e];
+
           // scores -> x (above), maximum, P'
           // (rows behind the tile's last one have Q = 0 and are never stored)
           const bool edge = t0 < all_lo || t0 + BN > all_hi || sg.masked;
-          float lv[NT / 2], inv[NT / 2];
-          float mx[2] = {-INFINITY, -INFINITY};
+          float inv[NG];
+          float mx[NQ][2];
 #pragma unroll
-          for (int kk = 0; kk < NT / 2; ++kk) {
-            const float ks_ = lds32f(sc + kk * 4), vs = usable_scale(lds32f(sc + (Tr::GROUPS + kk) * 4));
-            lv[kk] = log2f(vs);
-            inv[kk] = 1.f / vs;
+          for (int nq = 0; nq < NQ; ++nq) mx[nq][0] = mx[nq][1] = -INFINITY;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              const float c1 = ks_ * mul[hf];
+          for (int g = 0; g < NG; ++g) {
+            const float ks_ = lds32f(sc + g * 4), vs = usable_scale(lds32f(sc + (Tr::GROUPS + g) * 4));
+            const float lv = log2f(vs);
+            inv[g] = 1.f / vs;
 #pragma unroll
-              for (int h2 = 0; h2 < 2; ++h2)
+            for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  float x = s_acc[2 * kk + h2][hf * 2 + e];
-                  if (has_softcap) {
-                    const float ex = __expf(2.f * (x * c1));
-                    x = cap_l2 * (1.f - __fdividef(2.f, ex + 1.f)) + lv[kk];
-                  } else {
-                    x = fmaf(x, c1, lv[kk]);
-                  }
-                  if (edge) {
-                    const int j = col0 + kk * 16 + h2 * 8 + 2 * t4 + e;
-                    if (j < row_lo[hf] || j > row_hi[hf]) x = -INFINITY;
-                  }
-                  s_acc[2 * kk + h2][hf * 2 + e] = x;
-                  mx[hf] = fmaxf(mx[hf], x);
+              for (int e = 0; e < 4; ++e) {
+                const int u = e & 1;
+                float x = s_acc[g][nq][e];
+                if (has_softcap) {
+                  const float ex = __expf(2.f * (x * (ks_ * mul[nq][u])));
+                  x = cap_l2 * (1.f - __fdividef(2.f, ex + 1.f)) + lv;
+                } else {
+                  x = fmaf(x, ks_ * mul[nq][u], lv);
                 }
-            }
-          }
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            float m = mx[hf];
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            m = fmaxf(m_run[hf], m);
-            const float m_use = m == -INFINITY ? 0.f : m - 15.f;
-            const float corr = fast_exp2(m_run[hf] - m);  // NaN while the row has seen nothing: nothing to rescale then
-            const bool moved = m_run[hf] != m && m_run[hf] != -INFINITY;
-            m_run[hf] = m;
-            float l = moved ? l_run[hf] * corr : l_run[hf];
-#pragma unroll
-            for (int kk = 0; kk < NT / 2; ++kk) {
-              float sum = 0.f;
-#pragma unroll
-              for (int h2 = 0; h2 < 2; ++h2)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float pv = fast_exp2(s_acc[2 * kk + h2][hf * 2 + e] - m_use);
-                  s_acc[2 * kk + h2][hf * 2 + e] = pv;
-                  sum += pv;
+                if (edge) {
+                  const int j = col0 + g * 16 + 8 * (e >> 1) + g8;
+                  if (j < row_lo[nq][u] || j > row_hi[nq][u]) x = -INFINITY;
                 }
-              l = fmaf(sum, inv[kk], l);
-            }
-            l_run[hf] = l;
-            if (moved) {
-#pragma unroll
-              for (int dt = 0; dt < DT; ++dt) {
-                o_acc[dt][hf * 2] *= corr;
-                o_acc[dt][hf * 2 + 1] *= corr;
+                s_acc[g][nq][e] = x;
+                mx[nq][u] = fmaxf(mx[nq][u], x);
               }
+          }
+          bool any_moved = false;
+          float corr[NQ][2];
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float m = mx[nq][u];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+              m = fmaxf(m_run[nq][u], m);
+              const float m_use = m == -INFINITY ? 0.f : m - 15.f;
+              const bool moved = m_run[nq][u] != m && m_run[nq][u] != -INFINITY;
+              corr[nq][u] = moved ? fast_exp2(m_run[nq][u] - m) : 1.f;
+              any_moved |= moved;
+              m_run[nq][u] = m;
+              float l = l_run[nq][u] * corr[nq][u];
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                const float p0 = fast_exp2(s_acc[g][nq][u] - m_use), p1 = fast_exp2(s_acc[g][nq][2 + u] - m_use);
+                s_acc[g][nq][u] = p0;
+                s_acc[g][nq][2 + u] = p1;
+                l = fmaf(p0 + p1, inv[g], l);
+              }
+              l_run[nq][u] = l;
             }
+          if (any_moved) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o_acc[dt][nq][e] *= corr[nq][e & 1];
           }
 
           // codes of keys that no row of the tile sees may be anything; 0 * NaN is NaN
           const bool cut = t0 < sq.key_lo || t0 + BN > sq.key_hi;
 #pragma unroll
-          for (int kk = 0; kk < NT / 2; ++kk) {
-            uint32_t a[4];
-            a[0] = pack2<__half>(s_acc[2 * kk][0], s_acc[2 * kk][1]);
-            a[1] = pack2<__half>(s_acc[2 * kk][2], s_acc[2 * kk][3]);
-            a[2] = pack2<__half>(s_acc[2 * kk + 1][0], s_acc[2 * kk + 1][1]);
-            a[3] = pack2<__half>(s_acc[2 * kk + 1][2], s_acc[2 * kk + 1][3]);
+          for (int g = 0; g < NG; ++g) {
+            uint32_t b[NQ][2];
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) {
+              b[nq][0] = transpose_8x8(pack2<__half>(s_acc[g][nq][0], s_acc[g][nq][1]));
+              b[nq][1] = transpose_8x8(pack2<__half>(s_acc[g][nq][2], s_acc[g][nq][3]));
+            }
 #pragma unroll
             for (int half = 0; half < Tr::HALVES; ++half) {
               uint32_t vw[4][4];  // key rows 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const int row = wn * Tr::NW + kk * 16 + 2 * t4 + (r & 1) + 8 * (r >> 1);
+                const int row = wn * Tr::NW + g * 16 + 2 * t4 + (r & 1) + 8 * (r >> 1);
                 if (Tr::ROWB == 128) lds128(vw[r], code_addr<Tr>(v_base, row, half * 8 + g8));
                 else lds64(vw[r], code_addr<Tr>(v_base, row, g8 >> 1) + (g8 & 1) * 8);
                 if (cut) {
@@ -425,13 +462,13 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
 #pragma unroll
               for (int e = 0; e < Tr::VB / 4; ++e) {
 #pragma unroll
-                for (int pr = 0; pr < 2; ++pr) {
+                for (int pr = 0; pr < 2; ++pr) {  // columns 4 e + 2 pr (tile row g8) and the next (tile row g8 + 8)
                   const uint32_t sel = pr == 0 ? 0x5140u : 0x7362u;
-                  uint32_t b0[2], b1[2];
-                  decode4<CODE>(__byte_perm(vw[0][e], vw[1][e], sel), b0[0], b0[1]);
-                  decode4<CODE>(__byte_perm(vw[2][e], vw[3][e], sel), b1[0], b1[1]);
+                  uint32_t a[4];
+                  decode4<CODE>(__byte_perm(vw[0][e], vw[1][e], sel), a[0], a[1]);
+                  decode4<CODE>(__byte_perm(vw[2][e], vw[3][e], sel), a[2], a[3]);
 #pragma unroll
-                  for (int q = 0; q < 2; ++q) mma_16816<__half>(o_acc[half * Tr::VB + e * 4 + pr * 2 + q], a, b0[q], b1[q]);
+                  for (int nq = 0; nq < NQ; ++nq) mma_16816<__half>(o_acc[half * (Tr::VB / 2) + e * 2 + pr][nq], a, b[nq][0], b[nq][1]);
                 }
               }
             }
@@ -443,55 +480,59 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
 
         // ---- merge of the WN key slices and output ----
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float l = l_run[hf];
-          l += __shfl_xor_sync(0xffffffffu, l, 1);
-          l += __shfl_xor_sync(0xffffffffu, l, 2);
-          if (t4 == 0) ml[wn * BM + wm * 16 + g8 + 8 * hf] = make_float2(m_run[hf], l);
-        }
-        asm volatile("bar.sync 1, %0;\n" ::"n"(NCT));
-        float f_row[2];
+        for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int trow = wm * 16 + g8 + 8 * hf;
-          float m_all = -INFINITY;
+          for (int u = 0; u < 2; ++u) {
+            float l = l_run[nq][u];
 #pragma unroll
-          for (int k = 0; k < WN; ++k) m_all = fmaxf(m_all, ml[k * BM + trow].x);
-          const float m_use = m_all == -INFINITY ? 0.f : m_all;
-          float l_all = 0.f;
-#pragma unroll
-          for (int k = 0; k < WN; ++k) {
-            const float2 x = ml[k * BM + trow];
-            l_all += x.y * fast_exp2(x.x - m_use);
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            if (g8 == 0) ml[wn * BM + (wm * NQ + nq) * 8 + 2 * t4 + u] = make_float2(m_run[nq][u], l);
           }
-          // only a sum of exactly 0 means that the row saw no key: a NaN stays one
-          f_row[hf] = l_all == 0.f ? 0.f : fast_exp2(m_run[hf] - m_use) / l_all;
-          if (wn == 0 && t4 == 0) s_lse[trow] = l_all == 0.f ? -INFINITY : (m_use - 15.f + log2f(l_all)) * kLn2;
-        }
-        // Slice 0 stores, the others add in turn: a fixed order.  n-tile t holds column t of every lane group's VB.
+        asm volatile("bar.sync 1, %0;\n" ::"n"(NCT));
+        float f_row[NQ][2];
+#pragma unroll
+        for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int trow = (wm * NQ + nq) * 8 + 2 * t4 + u;
+            float m_all = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < WN; ++k) m_all = fmaxf(m_all, ml[k * BM + trow].x);
+            const float m_use = m_all == -INFINITY ? 0.f : m_all;
+            float l_all = 0.f;
+#pragma unroll
+            for (int k = 0; k < WN; ++k) {
+              const float2 x = ml[k * BM + trow];
+              l_all += x.y * fast_exp2(x.x - m_use);
+            }
+            // only a sum of exactly 0 means that the row saw no key: a NaN stays one
+            f_row[nq][u] = l_all == 0.f ? 0.f : fast_exp2(m_run[nq][u] - m_use) / l_all;
+            if (wn == 0 && g8 == 0) s_lse[trow] = l_all == 0.f ? -INFINITY : (m_use - 15.f + log2f(l_all)) * kLn2;
+          }
+        // Slice 0 stores, the others add in turn: a fixed order.  Tile dt of a half holds columns 2 dt and 2 dt + 1 of every lane group's VB.
 #pragma unroll
         for (int half = 0; half < Tr::HALVES; ++half) {
 #pragma unroll 1
           for (int turn = 0; turn < WN; ++turn) {
             if (wn == turn) {
 #pragma unroll
-              for (int hf = 0; hf < 2; ++hf) {
-                float* dst = slab + (wm * 16 + g8 + 8 * hf) * Tr::SLAB_LD;
-                const float f = f_row[hf];
+              for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int u = 0; u < 2; ++u) {
+                  float* dst = slab + ((wm * NQ + nq) * 8 + 2 * t4 + u) * Tr::SLAB_LD + g8 * Tr::VB;
+                  const float f = f_row[nq][u];
 #pragma unroll
                   for (int e4 = 0; e4 < Tr::VB / 4; ++e4) {
-                    float4* q4 = reinterpret_cast<float4*>(dst + (2 * t4 + n) * Tr::VB + e4 * 4);
-                    const int dt = half * Tr::VB + e4 * 4, c = hf * 2 + n;
-                    float4 v = make_float4(o_acc[dt][c] * f, o_acc[dt + 1][c] * f, o_acc[dt + 2][c] * f, o_acc[dt + 3][c] * f);
+                    float4* q4 = reinterpret_cast<float4*>(dst + e4 * 4);
+                    const int dt = half * (Tr::VB / 2) + e4 * 2;
+                    float4 v = make_float4(o_acc[dt][nq][u] * f, o_acc[dt][nq][2 + u] * f, o_acc[dt + 1][nq][u] * f, o_acc[dt + 1][nq][2 + u] * f);
                     if (turn > 0) {
                       const float4 old = *q4;
                       v.x += old.x; v.y += old.y; v.z += old.z; v.w += old.w;
                     }
                     *q4 = v;
                   }
-              }
+                }
             }
             asm volatile("bar.sync 1, %0;\n" ::"n"(NCT));
           }

@@ -39,7 +39,6 @@ struct Kv8Plan {
   Kv8TileInfo tile;
   int hd, grid;
   bool tiled;
-  int subs;  // tile kernel: sub-tiles
   size_t lse_bytes, workspace_bytes;
 };
 
@@ -110,8 +109,7 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   const int rows_max = a.seqlen_q * p.group;
   out->hd = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
   out->tiled = rows_max > 32;
-  out->subs = rows_max > 128 && out->hd <= 128 ? 2 : 1;
-  out->tile = out->tiled ? kv8_tile_info(out->hd, out->subs) : kv8_decode_info(out->hd, rows_max <= 8 ? 8 : rows_max <= 16 ? 16 : 32);
+  out->tile = out->tiled ? kv8_tile_info(out->hd, rows_max > 128 && out->hd <= 128 ? 256 : 128) : kv8_decode_info(out->hd, rows_max <= 8 ? 8 : rows_max <= 16 ? 16 : 32);
   const Kv8TileInfo& t = out->tile;
   p.m_blocks = std::max(1, ceil_div(rows_max, t.block_m));
   p.box_rows = t.block_n;
@@ -132,8 +130,9 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
     if (units < slots) ns = (int)std::max<long long>(1, std::min<long long>(slots / units, max_blocks / 8));
   } else if (max_blocks >= 4) {
     p.persistent = 1;
-    ns = 4;
-    if (slots / units > 3) ns = (int)std::max<long long>(4, std::min<long long>(slots / units + 2, max_blocks / 2 + 1));
+    // Partial slots of a unit.  They bound how finely the longest sequence is cut: with a slot for every CTA that an average unit gets, two
+    // thirds of the chip waited for a sequence twice as long as the others.
+    ns = (int)std::max<long long>(4, std::min<long long>(2 * slots / units + 3, max_blocks / 2 + 1));
   }
   if (!p.persistent) {
     p.blocks_per_split = ceil_div(max_blocks, ns);
@@ -179,9 +178,10 @@ static int run_kv8_fwd(const fa_fwd_params& a_in, const fa_kv8_cache& c, void* w
   }
   cudaError_t e;
   if (P.tiled) {
-    auto* launch = P.hd == 64    ? (P.subs == 1 ? launch_kv8_tile_64_1 : launch_kv8_tile_64_2)
-                   : P.hd == 128 ? (P.subs == 1 ? launch_kv8_tile_128_1 : launch_kv8_tile_128_2)
-                                 : launch_kv8_tile_256_1;
+    const bool small = P.tile.block_m == 128;
+    auto* launch = P.hd == 64    ? (small ? launch_kv8_tile_64_128 : launch_kv8_tile_64_256)
+                   : P.hd == 128 ? (small ? launch_kv8_tile_128_128 : launch_kv8_tile_128_256)
+                                 : launch_kv8_tile_256_128;
     e = launch(p, P.grid, st);
   } else {
     CUtensorMap tm_k, tm_v;

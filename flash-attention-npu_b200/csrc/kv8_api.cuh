@@ -20,13 +20,13 @@ FA_KV8_LAUNCHER(launch_kv8_decode_256_e4m3)
 FA_KV8_LAUNCHER(launch_kv8_decode_256_int8)
 #undef FA_KV8_LAUNCHER
 
-// Tile kernel: `subs` sub-tiles of 128 rows, 1 or (up to 128 columns) 2.
-Kv8TileInfo kv8_tile_info(int hd, int subs);
-cudaError_t launch_kv8_tile_64_1(const Kv8Params& p, int grid, cudaStream_t st);
-cudaError_t launch_kv8_tile_64_2(const Kv8Params& p, int grid, cudaStream_t st);
-cudaError_t launch_kv8_tile_128_1(const Kv8Params& p, int grid, cudaStream_t st);
-cudaError_t launch_kv8_tile_128_2(const Kv8Params& p, int grid, cudaStream_t st);
-cudaError_t launch_kv8_tile_256_1(const Kv8Params& p, int grid, cudaStream_t st);
+// Tile kernel: tiles of 128 or (up to 128 columns) 256 rows.
+Kv8TileInfo kv8_tile_info(int hd, int rows);
+cudaError_t launch_kv8_tile_64_128(const Kv8Params& p, int grid, cudaStream_t st);
+cudaError_t launch_kv8_tile_64_256(const Kv8Params& p, int grid, cudaStream_t st);
+cudaError_t launch_kv8_tile_128_128(const Kv8Params& p, int grid, cudaStream_t st);
+cudaError_t launch_kv8_tile_128_256(const Kv8Params& p, int grid, cudaStream_t st);
+cudaError_t launch_kv8_tile_256_128(const Kv8Params& p, int grid, cudaStream_t st);
 
 cudaError_t launch_kv8_append(const fa_kv8_append_params& p, int num_sm, int32_t* status, cudaStream_t st);
 cudaError_t launch_kv8_append_dense(const Kv8Params& p, cudaStream_t st);

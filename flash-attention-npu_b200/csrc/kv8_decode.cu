@@ -14,10 +14,10 @@ static Kv8TileInfo decode_info(int rows) {
 }
 Kv8TileInfo kv8_decode_info(int hd, int rows) { return hd == 64 ? decode_info<64>(rows) : hd == 128 ? decode_info<128>(rows) : decode_info<256>(rows); }
 
-Kv8TileInfo kv8_tile_info(int hd, int subs) {
-  if (hd == 64) return subs == 1 ? info<Kv8TileTraits<64, 1>>() : info<Kv8TileTraits<64, 2>>();
-  if (hd == 128) return subs == 1 ? info<Kv8TileTraits<128, 1>>() : info<Kv8TileTraits<128, 2>>();
-  return info<Kv8TileTraits<256, 1>>();
+Kv8TileInfo kv8_tile_info(int hd, int rows) {
+  if (hd == 64) return rows == 128 ? info<Kv8TileTraits<64, 2, true>>() : info<Kv8TileTraits<64, 2, false>>();
+  if (hd == 128) return rows == 128 ? info<Kv8TileTraits<128, 2, true>>() : info<Kv8TileTraits<128, 2, false>>();
+  return info<Kv8TileTraits<256, 1, false>>();
 }
 
 }  // namespace fa

@@ -1,4 +1,5 @@
 #define FA_INST_HD 128
 #define FA_INST_NSUB 2
-#define FA_INST_NAME launch_kv8_tile_128_2
+#define FA_INST_DUAL true
+#define FA_INST_NAME launch_kv8_tile_128_128
 #include "kv8_tile_inst.inc"

@@ -1,4 +1,5 @@
 #define FA_INST_HD 64
 #define FA_INST_NSUB 2
-#define FA_INST_NAME launch_kv8_tile_64_2
+#define FA_INST_DUAL false
+#define FA_INST_NAME launch_kv8_tile_64_256
 #include "kv8_tile_inst.inc"

@@ -6,30 +6,33 @@
 // was (the prefix sum goes on as if it had been served, so that the pages taken are always the list's first ones).
 //
 // Latency-bound: a few bytes a token.  One launch: every CTA sums up all requests by itself (two prefix sums of b entries, from L2)
-// and then writes its share of the tokens and of the table, so no CTA waits for another.
+// and then writes its share of the tokens and of the table, a token a thread up to a CTA for every SM, so no CTA waits for another.
+// 1024 requests with 33000 tokens: 6.1 us (with four tokens a thread and divisions of 64 bits 12.4); 8 requests 3.6.
 #include <algorithm>
 
 #include "common.cuh"
 
 namespace fa {
 
-constexpr int kPlanThreads = 256, kPlanTokens = 4 * kPlanThreads;
+constexpr int kPlanThreads = 256;
 
 struct PlanRequest {
   int64_t have, add;
   int had, need;
   bool fits;
 };
-__device__ __forceinline__ PlanRequest plan_request(const fa_kvcache_plan_params& p, int r) {
+__device__ __forceinline__ PlanRequest plan_request(const fa_kvcache_plan_params& p, int have, int add) {
   PlanRequest q;
-  q.have = p.have[r];
-  q.add = p.add[r];
-  q.fits = q.have >= 0 && q.add >= 0 && q.have + q.add <= (int64_t)p.cols * p.page_size;
-  q.add = max(q.add, (int64_t)0);
-  q.had = q.fits ? (int)((q.have + p.page_size - 1) / p.page_size) : 0;
-  q.need = q.fits ? (int)((q.have + q.add + p.page_size - 1) / p.page_size) - q.had : 0;
+  q.have = have;
+  q.add = max(add, 0);
+  const int64_t after = q.have + q.add;
+  q.fits = have >= 0 && add >= 0 && after <= (int64_t)p.cols * p.page_size;  // (which is within 32 bits)
+  auto pages = [&](uint32_t n) { return n == 0 ? 0 : (int)((n - 1) / (uint32_t)p.page_size) + 1; };  // (32 bits: a division of 64 is a call)
+  q.had = q.fits ? pages((uint32_t)have) : 0;
+  q.need = q.fits ? pages((uint32_t)after) - q.had : 0;
   return q;
 }
+__device__ __forceinline__ PlanRequest plan_request(const fa_kvcache_plan_params& p, int r) { return plan_request(p, p.have[r], p.add[r]); }
 
 __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid_constant__ fa_kvcache_plan_params p, int32_t* status) {
   extern __shared__ int2 s_pre[];  // per request: tokens and pages in front of it; [b]: of all
@@ -39,11 +42,22 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = ceil_div(p.b, kPlanThreads), r0 = min(p.b, tid * per), r1 = min(p.b, r0 + per);
   int2 sum = make_int2(0, 0);
-  for (int r = r0; r < r1; ++r) {
-    const PlanRequest q = plan_request(p, r);
-    s_pre[r] = sum;
-    sum.x += (int)q.add;
-    sum.y += q.need;
+  for (int rb = r0; rb < r1; rb += 4) {
+    int have[4], add[4];  // (all on their way before the first is used)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = min(rb + k, r1 - 1);
+      have[k] = p.have[r];
+      add[k] = p.add[r];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (rb + k >= r1) break;
+      const PlanRequest q = plan_request(p, have[k], add[k]);
+      s_pre[rb + k] = sum;
+      sum.x += (int)q.add;
+      sum.y += q.need;
+    }
   }
   int2 incl = sum;
 #pragma unroll
@@ -105,7 +119,7 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
       const int64_t at = q.have + (t - s_pre[lo].x);
       pos = (int)at;
       if (granted(q, lo) && at >= 0 && at < q.have + q.add) {
-        const int col = (int)(at / p.page_size), in = (int)(at - (int64_t)col * p.page_size);
+        const int col = (int)((uint32_t)at / (uint32_t)p.page_size), in = (int)at - col * p.page_size;
         const int page = col < q.had ? p.table[(int64_t)lo * p.table_stride + col] : p.free_pages[s_pre[lo].y + col - q.had];
         slot = (int64_t)page * p.page_size + in;
       }
@@ -116,8 +130,8 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
 }
 
 cudaError_t launch_kvcache_plan(const fa_kvcache_plan_params& p, int num_sm, int32_t* status, cudaStream_t st) {
-  int64_t grid = (p.total + kPlanTokens - 1) / kPlanTokens;
-  grid = std::max<int64_t>(grid, ceil_div(p.b, 4 * (kPlanThreads / 32)));
+  int64_t grid = (p.total + kPlanThreads - 1) / kPlanThreads;
+  grid = std::max<int64_t>(grid, ceil_div(p.b, kPlanThreads / 32));
   grid = std::min<int64_t>(std::max<int64_t>(grid, 1), num_sm);
   const size_t smem = (size_t)(p.b + 1) * sizeof(int2);
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kvcache_plan_kernel), (FA_B200_PLAN_MAX_REQUESTS + 1) * (int)sizeof(int2));

@@ -113,8 +113,10 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   const Kv8TileInfo& t = out->tile;
   p.m_blocks = std::max(1, ceil_div(rows_max, t.block_m));
   p.box_rows = t.block_n;
-  if (a.block_table)
-    while (a.page_size % p.box_rows != 0) p.box_rows >>= 1;  // (16 divides the page)
+  if (a.block_table && a.page_size % p.box_rows != 0) {
+    p.box_rows &= -p.box_rows;  // a power of two divides the stage ...
+    while (a.page_size % p.box_rows != 0) p.box_rows >>= 1;  // ... and the page (16 does)
+  }
   long long range = a.seqlen_k;
   if (is_local && wl >= 0) range = std::min<long long>(range, (long long)wl + std::max(wr, 0) + ceil_div(t.block_m, p.group) + 1);
   const int max_blocks = std::max(1, std::min(ceil_div((int)range, t.block_n) + 1, ceil_div(a.seqlen_k, t.block_n)));

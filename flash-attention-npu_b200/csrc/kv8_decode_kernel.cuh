@@ -29,10 +29,10 @@ namespace fa {
 
 template <int HD_, int WM_, int NQ_>
 struct Kv8Traits {
-  static constexpr int HD = HD_, WM = WM_, NQ = NQ_, WN = 4, NCW = WM * WN;  // NQ: 8-row tiles of a warp; WM warps' rows, WN warps' keys
+  static constexpr int HD = HD_, WM = WM_, NQ = NQ_, WN = HD == 128 && WM == 2 ? 5 : 4, NCW = WM * WN;  // NQ: 8-row tiles of a warp; WM warps' rows, WN warps' keys
   static_assert(HD == 64 || HD == 128 || HD == 256, "tile widths; a head dim below the width leaves zero columns (TMA fill)");
   static constexpr int BM = 8 * NQ * WM;
-  static constexpr int BN = HD == 256 ? 64 : 128;
+  static constexpr int BN = HD == 256 ? 64 : 32 * WN;
   static constexpr int NTHREADS = 32 * (NCW + 1);
   static constexpr int NW = BN / WN;   // keys of a consumer warp in a stage
   static constexpr int NG = NW / kScaleGranule;  // 16-key groups of them

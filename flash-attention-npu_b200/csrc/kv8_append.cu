@@ -55,14 +55,23 @@ __device__ __forceinline__ void unpack_pair(uint32_t w, float& a, float& b) {
     b = f.y;
   }
 }
-// Running maximum of |element| per half word; NaN has no part in it.
-template <typename T>
+// Running maximum of |element| per half word: NaN when one is (NAN_TOO), or as if none were.
+template <typename T, bool NAN_TOO>
 __device__ __forceinline__ uint32_t abs_max2(uint32_t mx, uint32_t w) {
   w &= 0x7fff7fffu;
   uint32_t r;
-  if (std::is_same<T, __nv_bfloat16>::value) asm("max.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
-  else asm("max.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
+  if (std::is_same<T, __nv_bfloat16>::value) {
+    if (NAN_TOO) asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
+    else asm("max.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
+  } else {
+    if (NAN_TOO) asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
+    else asm("max.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(mx), "r"(w));
+  }
   return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max8(uint32_t mx, const uint4& x) {
+  return abs_max2<T, true>(abs_max2<T, true>(abs_max2<T, true>(abs_max2<T, true>(mx, x.x), x.y), x.z), x.w);
 }
 // A pair with its infinities taken out.
 template <typename T>
@@ -104,20 +113,21 @@ __device__ __forceinline__ void write_run(Load load, uint8_t* dst, int64_t row_s
   for (int r0 = my.row + more; r0 < rows; r0 += more) {  // (the first batch last: it stays)
     fetch(r0);
 #pragma unroll
-    for (int k = 0; k < BATCH; ++k) mx = abs_max2<T>(abs_max2<T>(abs_max2<T>(abs_max2<T>(mx, keep[k].x), keep[k].y), keep[k].z), keep[k].w);
+    for (int k = 0; k < BATCH; ++k) mx = abs_max8<T>(mx, keep[k]);
   }
   fetch(my.row);
 #pragma unroll
-  for (int k = 0; k < BATCH; ++k) mx = abs_max2<T>(abs_max2<T>(abs_max2<T>(abs_max2<T>(mx, keep[k].x), keep[k].y), keep[k].z), keep[k].w);
+  for (int k = 0; k < BATCH; ++k) mx = abs_max8<T>(mx, keep[k]);
   float lo, hi;
   unpack_pair<T>(mx, lo, hi);
-  if (fmaxf(lo, hi) == INFINITY) {  // rare: the maximum without the infinities
+  const bool finite = lo < INFINITY && hi < INFINITY;
+  if (!finite) {  // rare: the maximum without infinities and NaN
     mx = 0;
 #pragma unroll 1
     for (int r = my.row; r < rows; r += my.step) {
       const uint4 x = load(r);
-      mx = abs_max2<T>(abs_max2<T>(mx, finite2<T>(x.x)), finite2<T>(x.y));
-      mx = abs_max2<T>(abs_max2<T>(mx, finite2<T>(x.z)), finite2<T>(x.w));
+      mx = abs_max2<T, false>(abs_max2<T, false>(mx, finite2<T>(x.x)), finite2<T>(x.y));
+      mx = abs_max2<T, false>(abs_max2<T, false>(mx, finite2<T>(x.z)), finite2<T>(x.w));
     }
     unpack_pair<T>(mx, lo, hi);
   }
@@ -170,13 +180,41 @@ __device__ __forceinline__ void write_run(Load load, uint8_t* dst, int64_t row_s
   if ((bits & 0x7fffffu) == 0 && exponent >= 1 && exponent <= 253) {  // a power of two: its reciprocal is exact
     const float inv = __uint_as_float((254u - exponent) << 23);
     auto by = [&](float v) { return __fmul_rn(v, inv); };
-    for (int r0 = my.row;;) {
+    auto all = [&](auto one) {
+      for (int r0 = my.row;;) {
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k)
-        if (r0 + k * my.step < rows) put(r0 + k * my.step, keep[k], by);
-      r0 += more;
-      if (r0 >= rows) break;
-      fetch(r0);
+        for (int k = 0; k < BATCH; ++k)
+          if (r0 + k * my.step < rows) one(r0 + k * my.step, keep[k]);
+        r0 += more;
+        if (r0 >= rows) break;
+        fetch(r0);
+      }
+    };
+    // Two fp16 elements at a time, where none is special and the reciprocal is a normal fp16: the product is exact (or so small that its code
+    // is 0 either way).  x / now + 1536 is rounded to a whole number, whose low byte is the code.  9800 tokens of seven prompts, 8 heads of
+    // 128, int8: 17.3 us one element after the other, 19 instructions each, 15.6 with this and the prefetch.
+    if (BATCH > 1 && std::is_same<T, __half>::value && finite && exponent >= 112 && exponent <= 141) {
+      const uint32_t inv2 = pack2<__half>(inv, inv);
+      all([&](int r, const uint4& x) {
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        uint32_t c[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (CODE == FA_CODE_E4M3) {
+            uint32_t y;
+            uint16_t z;
+            asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(y) : "r"(w[e]), "r"(inv2));
+            asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;\n" : "=h"(z) : "r"(y));
+            c[e] = z;
+          } else {
+            asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(c[e]) : "r"(w[e]), "r"(inv2), "r"(0x66006600u));
+          }
+        }
+        constexpr uint32_t sel = CODE == FA_CODE_E4M3 ? 0x5410 : 0x6420;
+        *reinterpret_cast<uint2*>(dst + (int64_t)r * row_stride) = make_uint2(__byte_perm(c[0], c[1], sel), __byte_perm(c[2], c[3], sel));
+      });
+    } else {
+      all([&](int r, const uint4& x) { put(r, x, by); });
     }
   } else {  // a scale that somebody else has chosen: rare, and kept short
 #pragma unroll 1
@@ -200,6 +238,19 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(const __g
   const uint32_t sb = (uint32_t)p.c.scale_block, blocks = (uint32_t)p.rows / sb;
   const int64_t slots = (int64_t)p.kv_outer * p.rows;  // below 2^31
   if (tid == 0) s_runs = 0;
+  // The window's elements are wanted whatever its slots say: on their way to L2 while those are looked up.
+  const int pairs = 2 * p.h_k;
+  const int mine = (pairs - blockIdx.y + gridDim.y - 1) / gridDim.y;  // every gridDim.y-th pair
+  if (window > 1 && mine > 1) {
+    const int lines = ceil_div(p.d, 64), here = (int)min((int64_t)window, p.total - t0);
+    for (int i = tid; i < here * mine * lines; i += kAppendThreads) {
+      const int line = i % lines, m = i / lines % mine, tok = i / lines / mine, pair = blockIdx.y + m * gridDim.y;
+      const bool is_v = pair & 1;
+      const T* x = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)(pair >> 1) * (is_v ? p.v_head_stride : p.k_head_stride) +
+                   (t0 + tok) * (is_v ? p.v_tok_stride : p.k_tok_stride) + line * 64;
+      asm volatile("prefetch.global.L2 [%0];\n" ::"l"(x));
+    }
+  }
   __syncthreads();
   if (tid < window && t0 + tid < p.total) {
     const int64_t s = p.slots[t0 + tid], before = t0 + tid > 0 ? p.slots[t0 + tid - 1] : -1;
@@ -252,8 +303,6 @@ __global__ void __launch_bounds__(kAppendThreads, 4) kv8_append_kernel(const __g
     write_run<T, CODE, decltype(group)::value, decltype(batch)::value>(load, codes + my.col * 8, row_stride, (int)(s % sb), s_len[r], my, scale, t, s_red);
   };
   using std::integral_constant;
-  const int pairs = 2 * p.h_k;
-  const int mine = (pairs - blockIdx.y + gridDim.y - 1) / gridDim.y;  // every gridDim.y-th pair
   for (int i = warp; i < runs * mine; i += kAppendWarps) {
     const int m = i / runs, r = i - m * runs, pair = blockIdx.y + m * gridDim.y, n = s_len[r] * chunks;
     if (n <= 32) run(integral_constant<int, 32>(), integral_constant<int, 1>(), r, pair, lane);
@@ -327,9 +376,14 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_dense_kernel(const 
 template <typename T, int CODE>
 static cudaError_t append_t(const fa_kv8_append_params& p, int num_sm, int32_t* status, cudaStream_t st) {
   // A window has as many tokens as leave every SM eight CTAs, up to a scale block, in which one run of a prompt starts: one for a
-  // decoding step, whose runs then lie side by side.  A CTA has one pair for long runs, eight for warps that write alone.
+  // decoding step, whose runs then lie side by side.  A CTA has eight pairs for warps that write alone and one for long runs; where runs may
+  // be long but the tokens are few, as many (up to four) as bring the CTAs into one wave, since they may be a decoding batch as well as a
+  // prompt (blocks of 128 tokens, 8 heads, one or as many pairs as the rule says: 64 requests 5.8 and 3.5 us, a prompt of 64 tokens 5.1
+  // and 5.4; 128 requests 10.2 and 3.7, a prompt 7.3 and 9.2).
   const int pairs = 2 * p.h_k, sb = p.c.scale_block;
-  const int groups = std::min<int64_t>(p.total, sb) * (p.d / 8) > kWarpRun ? pairs : (pairs + kAppendWarps - 1) / kAppendWarps;
+  const bool maybe_long = std::min<int64_t>(p.total, sb) * (p.d / 8) > kWarpRun;
+  const int64_t waves = (p.total * pairs + 4LL * num_sm - 1) / (4LL * num_sm);
+  const int each = !maybe_long ? kAppendWarps : waves > 4 ? 1 : (int)waves, groups = (pairs + each - 1) / each;
   const int most = std::min(kMaxWindow, sb);
   const int window = (int)std::min<int64_t>(most, std::max<int64_t>(1, p.total * groups / (8LL * num_sm)));
   const dim3 grid((unsigned)((p.total + window - 1) / window), (unsigned)groups);

@@ -423,20 +423,20 @@ static int make_plan(const fa_fwd_params& a_in, Planned* out, const fa_fwd_plan*
 // The merge kernel is launched as a programmatic dependent (launch_dependent, common.cuh): the launch itself and the start of
 // its CTAs overlap the tail of the split-KV attention kernel in front of it, which hides most of what a second launch costs.
 template <typename OutT>
-static cudaError_t launch_combine_t(const fa_combine_params& c, int64_t rows, cudaStream_t st) {
+static cudaError_t launch_combine_t(const fa_combine_params& c, const int32_t* rows_end, int64_t rows, cudaStream_t st) {
   const bool wide = c.num_splits > 32;
-  if (wide) return launch_dependent(combine_wide_kernel<OutT>, dim3((unsigned)rows), kCombineWideWarps * 32, 0, st, c);
-  return launch_dependent(combine_kernel<OutT>, dim3((unsigned)((rows + kCombineWarps - 1) / kCombineWarps)), kCombineWarps * 32, 0, st, c);
+  if (wide) return launch_dependent(combine_wide_kernel<OutT>, dim3((unsigned)rows), kCombineWideWarps * 32, 0, st, c, rows_end);
+  return launch_dependent(combine_kernel<OutT>, dim3((unsigned)((rows + kCombineWarps - 1) / kCombineWarps)), kCombineWarps * 32, 0, st, c, rows_end);
 }
 
-static int launch_combine(const fa_combine_params& c, cudaStream_t st) {
+static int launch_combine(const fa_combine_params& c, cudaStream_t st, const int32_t* rows_end = nullptr) {
   const int64_t rows = (int64_t)c.b * c.s * c.h;
   if (rows == 0) return FA_OK;
   if (rows > 0x7fffffffLL) return fail(FA_ERR_UNSUPPORTED, "too many rows to merge");
   cudaError_t e;
-  if (c.out_dtype == FA_BF16) e = launch_combine_t<__nv_bfloat16>(c, rows, st);
-  else if (c.out_dtype == FA_FP16) e = launch_combine_t<__half>(c, rows, st);
-  else if (c.out_dtype == 2) e = launch_combine_t<float>(c, rows, st);
+  if (c.out_dtype == FA_BF16) e = launch_combine_t<__nv_bfloat16>(c, rows_end, rows, st);
+  else if (c.out_dtype == FA_FP16) e = launch_combine_t<__half>(c, rows_end, rows, st);
+  else if (c.out_dtype == 2) e = launch_combine_t<float>(c, rows_end, rows, st);
   else return fail(FA_ERR_INVALID, "bad out_dtype");
   if (e != cudaSuccess) return fail(FA_ERR_CUDA, std::string("combine launch: ") + cudaGetErrorString(e));
   ++g_launches;
@@ -444,7 +444,7 @@ static int launch_combine(const fa_combine_params& c, cudaStream_t st) {
 }
 
 // for kv8_api.cu
-int merge_partials(const fa_combine_params& c, cudaStream_t st) { return launch_combine(c, st); }
+int merge_partials(const fa_combine_params& c, const int32_t* rows_end, cudaStream_t st) { return launch_combine(c, st, rows_end); }
 void window_rule(int seqlen_q, int max_k, bool causal, int& wl, int& wr, bool& is_causal, bool& is_local) {
   normalize_window(seqlen_q, max_k, causal, wl, wr, is_causal, is_local);
 }

@@ -76,9 +76,9 @@ __device__ __forceinline__ void merge_store_lse(const fa_combine_params& p, int 
   p.lse[bb * p.lse_batch_stride + ss * p.lse_row_stride + hh * p.lse_head_stride] = v;
 }
 
-// Up to 32 partials: one warp per output row.
+// Up to 32 partials: one warp per output row.  rows_end (or null): packed rows from *rows_end on belong to no sequence and stay as they were.
 template <typename OutT>
-__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __grid_constant__ fa_combine_params p) {
+__global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __grid_constant__ fa_combine_params p, const int32_t* rows_end) {
   grid_wait();
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * kCombineWarps + (threadIdx.x >> 5);
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
   const int hh = (int)(row % p.h);
   const int ss = (int)((row / p.h) % p.s);
   const int bb = (int)(row / ((int64_t)p.h * p.s));
+  if (rows_end && ss >= *rows_end) return;
   const float* lp = p.lse_partial + bb * p.lp_batch_stride + ss * p.lp_row_stride + hh * p.lp_head_stride;
   const float* op = p.o_partial + bb * p.op_batch_stride + ss * p.op_row_stride + hh * p.op_head_stride;
   OutT* out = reinterpret_cast<OutT*>(p.o) + bb * p.o_batch_stride + ss * p.o_row_stride + hh * p.o_head_stride;
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const __gri
 // warp per row 298 partials are a chain of ~300 dependent loads.
 constexpr int kCombineWideWarps = 16;
 template <typename OutT>
-__global__ void __launch_bounds__(kCombineWideWarps * 32) combine_wide_kernel(const __grid_constant__ fa_combine_params p) {
+__global__ void __launch_bounds__(kCombineWideWarps * 32) combine_wide_kernel(const __grid_constant__ fa_combine_params p, const int32_t* rows_end) {
   grid_wait();
   __shared__ float s_red[kCombineWideWarps];
   __shared__ float4 s_acc[kCombineWideWarps][32];
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kCombineWideWarps * 32) combine_wide_kernel(co
   const int hh = (int)(blockIdx.x % p.h);
   const int ss = (int)((blockIdx.x / p.h) % p.s);
   const int bb = (int)(blockIdx.x / ((int64_t)p.h * p.s));
+  if (rows_end && ss >= *rows_end) return;
   const float* lp = p.lse_partial + bb * p.lp_batch_stride + ss * p.lp_row_stride + hh * p.lp_head_stride;
   const float* op = p.o_partial + bb * p.op_batch_stride + ss * p.op_row_stride + hh * p.op_head_stride;
   OutT* out = reinterpret_cast<OutT*>(p.o) + bb * p.o_batch_stride + ss * p.o_row_stride + hh * p.o_head_stride;

@@ -13,7 +13,7 @@ namespace fa {
 // api.cu
 int fail_bwd(int code, const std::string& msg);
 void count_launches(int n);
-int merge_partials(const fa_combine_params& c, cudaStream_t st);
+int merge_partials(const fa_combine_params& c, const int32_t* rows_end, cudaStream_t st);
 void window_rule(int seqlen_q, int max_k, bool causal, int& wl, int& wr, bool& is_causal, bool& is_local);
 int sm_count();
 void clear_error();
@@ -64,6 +64,7 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   if (a.k_new && a.seqlen_new <= 0) return fail(FA_ERR_INVALID, "seqlen_new must be positive when k, v are given");
   if (!a.k_new && a.seqlen_new != 0) return fail(FA_ERR_INVALID, "seqlen_new given without k, v");
   if (a.k_new && !a.seqused_k) return fail(FA_ERR_INVALID, "appending k, v needs cache_seqlens");
+  if ((2LL * a.seqlen_new / kScaleGranule + 4) * a.b * a.h_k > 0x3fffffffLL) return fail(FA_ERR_UNSUPPORTED, "too many new tokens in one call");
   if (a.seqlen_new > a.seqlen_k) return fail(FA_ERR_INVALID, "the new tokens do not fit into the KV cache");
   if ((a.rotary_cos != nullptr) != (a.rotary_sin != nullptr)) return fail(FA_ERR_INVALID, "rotary_cos and rotary_sin must be passed together");
   if (a.rotary_cos) {
@@ -108,7 +109,7 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   // ---- tile and key splits ----
   const int rows_max = a.seqlen_q * p.group;
   out->hd = a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256;
-  out->tiled = rows_max > 32;
+  out->tiled = rows_max > 32;  // (both sides measured: kv8_decode_kernel.cuh)
   out->tile = out->tiled ? kv8_tile_info(out->hd, rows_max > 128 && out->hd <= 128 ? 256 : 128) : kv8_decode_info(out->hd, rows_max <= 8 ? 8 : rows_max <= 16 ? 16 : 32);
   const Kv8TileInfo& t = out->tile;
   p.m_blocks = std::max(1, ceil_div(rows_max, t.block_m));
@@ -144,7 +145,7 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   out->grid = (int)(p.persistent ? std::max(1LL, slots / a.h_k) * a.h_k : units * ns);
   const bool varlen = a.cu_seqlens_q != nullptr;
   p.lse_elems = varlen ? (int64_t)a.h * a.total_q : (int64_t)a.b * a.h * a.seqlen_q;
-  if (varlen ? a.lse_head_stride != a.total_q : (a.lse_head_stride != a.seqlen_q || a.lse_batch_stride != (int64_t)a.h * a.seqlen_q))
+  if (p.lse_elems > 0 && (varlen ? a.lse_head_stride != a.total_q : (a.lse_head_stride != a.seqlen_q || a.lse_batch_stride != (int64_t)a.h * a.seqlen_q)))
     return fail(FA_ERR_INVALID, "lse must be contiguous");
   if (ns > 1) {
     out->lse_bytes = ((size_t)ns * p.lse_elems * sizeof(float) + 15) & ~(size_t)15;
@@ -155,13 +156,13 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
 
 static int run_kv8_fwd(const fa_fwd_params& a_in, const fa_kv8_cache& c, void* ws, size_t ws_bytes, void* (*alloc)(size_t, void*), void* ctx,
                        cudaStream_t st) {
-  if (!a_in.q || !a_in.k || !a_in.v || !a_in.o || !a_in.lse) return fail(FA_ERR_INVALID, "q, k, v, o and lse must be non-null");
+  const bool no_rows = a_in.total_q == 0 || a_in.seqlen_q == 0;  // (new tokens are appended all the same)
+  if (!a_in.k || !a_in.v || (!no_rows && (!a_in.q || !a_in.o || !a_in.lse))) return fail(FA_ERR_INVALID, "q, k, v, o and lse must be non-null");
   Kv8Plan P;
   if (int rc = make_kv8_plan(a_in, c, &P); rc != FA_OK) return rc;
   Kv8Params& p = P.p;
   const fa_fwd_params& a = p.a;
-  if (a.total_q == 0 || a.seqlen_q == 0) return FA_OK;
-  if (P.workspace_bytes) {
+  if (P.workspace_bytes && !no_rows) {
     if (!ws && alloc) {
       ws = alloc(P.workspace_bytes, ctx);
       ws_bytes = ws ? P.workspace_bytes : 0;
@@ -178,6 +179,7 @@ static int run_kv8_fwd(const fa_fwd_params& a_in, const fa_kv8_cache& c, void* w
     if (e != cudaSuccess) return cuda_fail("append launch", e);
     count_launches(1);
   }
+  if (no_rows) return FA_OK;
   cudaError_t e;
   if (P.tiled) {
     const bool small = P.tile.block_m == 128;
@@ -225,7 +227,7 @@ static int run_kv8_fwd(const fa_fwd_params& a_in, const fa_kv8_cache& c, void* w
   m.o_row_stride = a.o_row_stride;
   m.o_head_stride = a.o_head_stride;
   m.out_dtype = a.dtype;
-  return merge_partials(m, st);
+  return merge_partials(m, varlen ? a.cu_seqlens_q + a.b : nullptr, st);
 }
 
 static int run_kv8_append(const fa_kv8_append_params& p_in, cudaStream_t st) {
@@ -244,7 +246,7 @@ static int run_kv8_append(const fa_kv8_append_params& p_in, cudaStream_t st) {
   if (!al16(p.k_cache) || !al16(p.v_cache) || !ok8(p.kc_outer_stride) || !ok8(p.kc_row_stride) || !ok8(p.kc_head_stride) ||
       !ok8(p.vc_outer_stride) || !ok8(p.vc_row_stride) || !ok8(p.vc_head_stride))
     return fail(FA_ERR_UNSUPPORTED, "the codes of an 8-bit KV cache must start at 16-byte boundaries, with strides that are multiples of 16");
-  if (p.total > 0x7fffffffLL || p.h_k > 65535) return fail(FA_ERR_UNSUPPORTED, "too many new tokens or heads in one call");
+  if (p.total > 0x7fffffffLL || p.h_k > 32767) return fail(FA_ERR_UNSUPPORTED, "too many new tokens or heads in one call");
   if ((int64_t)p.kv_outer * p.rows > 0x7fffffffLL) return fail(FA_ERR_UNSUPPORTED, "too many tokens in the KV cache");
   const int num_sm = p.num_sm > 0 ? p.num_sm : sm_count();
   int32_t* status = device_status_word();

@@ -1,8 +1,14 @@
-// Attention over an 8-bit KV cache for few query rows (the rows of a kv head's query group share a tile of 16 or 32).
+// Attention over an 8-bit KV cache for few query rows: the rows of a kv head's query group share a tile of 8, 16 or 32, the whole of a
+// sequence's.
 //
 // HBM-bound: K and V of the visible range are read once, at one byte per element.  A producer warp moves stages of BN keys
-// (K and V) with tiled TMA loads into a ring, and the stage's scales with 4-byte asynchronous copies; consumer warps own 16 query
-// rows and a slice of the stage's keys each, turn codes into fp16 in registers and multiply with mma.sync.
+// (K and V) with tiled TMA loads into a ring, and the stage's scales with 4-byte asynchronous copies; consumer warps own 8 or 16 query
+// rows and a slice of the stage's keys each, turn codes into fp16 in registers and multiply with mma.sync (the tile kernel on such calls:
+// 2.2 times as long for 8 rows, 7 % longer for 32; its 128-row tensor instruction waits for the turning of codes all the same).
+// 8 sequences of 131072 keys, 64 / 8 heads of 128: 313 us, 6.85 TB/s.  64 ragged ones of up to 8191 keys with a token appended: 109 us, 5.6
+// TB/s.  32 sequences with a window of 4096 keys and 4 tokens, 64 / 8 heads: 124 us of 40 that HBM would take -- at 32 rows a warp scheduler
+// holds three warps of 168 registers, and what they wait for is one another's products and the instruction cache, not memory (ncu: issue 37
+// %, mma 25 %); eight key slices of 32 rows each, with every code turned once, spill and took 205 us.
 //
 // Arithmetic.  K = ck * sk(block), V = cv * sv(block).  With the running maximum over x_j = scale * log2e * sk * (q . ck_j) + log2 sv,
 //   P'_j = 2^(x_j - m + 15),   O = sum_j P'_j cv_j / l,   l = sum_j P'_j / sv_j,   LSE = ln2 (m - 15) + ln l:
@@ -11,7 +17,7 @@
 // are fp16 values, sums and statistics are fp32.
 //
 // Both products are transposed, S^T = K Q^T and O^T = V^T P^T: query rows are the narrow side of mma m16n8k16, so that the eight rows
-// of a usual query group fill it (with rows on the wide side half of every product was padding).  P^T comes out of S^T by a transposition
+// of a usual query group fill it (rows on the wide side: 8 % faster at 32 rows, half of every product padding at 8; one short sequence 13.5 us against 11.3).  P^T comes out of S^T by a transposition
 // of 8 x 8 tiles within the warp (movmatrix).
 // Fragments straight from the codes.  A contraction may run over its index in any order, and output columns may be numbered in
 // any order, as long as both operands agree: lane (g8, t4) takes LB consecutive bytes of key rows g8 and g8 + 8 as the K elements of
@@ -44,7 +50,9 @@ struct Kv8Traits {
   static constexpr int HALF_BYTES = BN * ROWB;
   static constexpr int KV_BYTES = HALVES * HALF_BYTES;
   static constexpr int STAGE_BYTES = 2 * KV_BYTES;
-  // up to 16 rows: two resident CTAs of 96 KiB rings (64 columns: 80 KiB); 32 rows: one CTA with all of it (64 columns: two)
+  // up to 16 rows: two resident CTAs of 96 KiB rings (64 columns: 80 KiB); 32 rows: one CTA with all of it (64 columns: two).
+  // 32 rows of 128 columns: five key slices, since ten consumer warps and the producer fill the warp schedulers' registers (four: 128 us against 124
+  // in the case above).
   static constexpr int RESIDENT = WM == 1 || HD == 64 ? 2 : 1;
   static constexpr int ST = HD == 64 ? 5 : WM == 1 ? 3 : 5;
   static constexpr int GROUPS = BN / kScaleGranule;
@@ -146,11 +154,11 @@ __device__ __forceinline__ void kv8_load_q(const Kv8Params& p, const Kv8Seq& sq,
   constexpr int LPR = Tr::HD / 8, RPW = 32 / LPR;  // lanes of a row, rows of a warp
   const int rows_total = sq.q_len * p.group, sub = lane / LPR, c8 = (lane % LPR) * 8;
   for (int r0 = warp * RPW; r0 < Tr::BM; r0 += Tr::NCW * RPW) {
-    const int row = r0 + sub, rr = sg.mb * Tr::BM + row;
+    const int row = r0 + sub;
     Vec16 x;
     x.u = make_uint4(0, 0, 0, 0);
-    if (rr < rows_total && c8 < p.a.d) {
-      const int i = rr / p.group, head = sg.hk * p.group + (rr - i * p.group);
+    if (row < rows_total && c8 < p.a.d) {
+      const int i = row / p.group, head = sg.hk * p.group + (row - i * p.group);
       const T* qrow = reinterpret_cast<const T*>(p.a.q) + (int64_t)sg.bi * p.a.q_batch_stride +
                       (int64_t)(sq.q_row0 + i) * p.a.q_row_stride + (int64_t)head * p.a.q_head_stride;
       x.u = kv8_q_chunk<T>(p, qrow, c8, sq.k_len, i, rot_per_token);
@@ -232,8 +240,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
     uint32_t it_base = 0;
     while (sg.valid) {
       if (sg.valid == 1) {
-        const Kv8Seq sq = kv8_seq(p, mask, sg.bi, sg.mb, BM);
-        if (sg.mb * BM < sq.q_len * p.group) {
+        const Kv8Seq sq = kv8_seq(p, mask, sg.bi, 0, BM);
+        if (sq.q_len > 0) {
           if (!kv8_producer<Tr>(p, sq, sg, &tm_k, &tm_v, pipe, scales, full0, empty0, it_base, lane, &s_abort)) break;
           it_base += (uint32_t)sg.cnt;
         }
@@ -259,8 +267,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
       const Kv8Seg sg = s_seg;
       asm volatile("bar.sync 1, %0;\n" ::"n"(NCT));  // ... and read by everybody
       if (!sg.valid) break;
-      const Kv8Seq sq = kv8_seq(p, mask, sg.bi, sg.mb, BM);
-      const int rows = min(BM, sq.q_len * p.group - sg.mb * BM);  // of this tile
+      const Kv8Seq sq = kv8_seq(p, mask, sg.bi, 0, BM);
+      const int rows = min(BM, sq.q_len * p.group);  // (one tile holds all that a sequence may have)
       if (sg.valid == 1 && rows > 0) {
         const bool per_token = mask.causal || mask.local;
         if (p.a.dtype == FA_BF16) kv8_load_q<Tr, __nv_bfloat16>(p, sq, sg, q_base, factor, per_token, warp, lane);
@@ -278,7 +286,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
             for (int e = 0; e < 4; ++e) o_acc[dt][nq][e] = 0.f;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int r = (wm * NQ + nq) * 8 + 2 * t4 + u, i = (sg.mb * BM + r) / p.group;
+            const int r = (wm * NQ + nq) * 8 + 2 * t4 + u, i = r / p.group;
             int lo = 0, hi = sq.k_len - 1;
             if (mask.causal) hi = min(hi, i + sq.koff);
             if (mask.local) {
@@ -300,11 +308,11 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
             for (int nq = 0; nq < NQ; ++nq) lds64(qf[ks][nq], q_frag + (nq * KS + ks) * 256);
         }
         // every row of the tile sees keys [all_lo, all_hi)
-        const int i_first = sg.mb * BM / p.group, i_last = (sg.mb * BM + rows - 1) / p.group;
+        const int i_last = (rows - 1) / p.group;
         int all_lo = 0, all_hi = sq.k_len;
-        if (mask.causal) all_hi = min(all_hi, i_first + sq.koff + 1);
+        if (mask.causal) all_hi = min(all_hi, sq.koff + 1);
         if (mask.local) {
-          all_hi = min(all_hi, i_first + sq.koff + mask.wr + 1);
+          all_hi = min(all_hi, sq.koff + mask.wr + 1);
           all_lo = max(0, i_last + sq.koff - mask.wl);
         }
 
@@ -539,7 +547,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ C
           for (int c = tid; c < BM * (Tr::ROWB / 4); c += NCT) {
             const int trow = c / (Tr::ROWB / 4), s4 = (c % (Tr::ROWB / 4)) * 4, c4 = half * Tr::ROWB + s4;
             if (trow >= rows) continue;
-            const int rr = sg.mb * BM + trow, i = rr / p.group, head = sg.hk * p.group + (rr - i * p.group);
+            const int i = trow / p.group, head = sg.hk * p.group + (trow - i * p.group);
             const int64_t lse_idx = (int64_t)sg.bi * p.a.lse_batch_stride + (int64_t)head * p.a.lse_head_stride + sq.q_row0 + i;
             const float lse_row = s_lse[trow];
             const bool dead = lse_row == -INFINITY;

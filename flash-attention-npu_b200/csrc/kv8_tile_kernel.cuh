@@ -8,21 +8,26 @@
 // fp16's end, and below 2^7 it has as many bits as a 16-bit output shows; so O is rescaled in TMEM a few times a tile and
 // not at every block.
 //
-// Warps: 4 per sub-tile of 128 rows  softmax, one thread per row (Q load, P, rescale of O, epilogue)
-//        4                           converters: codes -> fp16 tiles in the swizzled operand layout; global loads of a tile in flight
-//                                    while the one before is turned
-//        1 per sub-tile              MMA issue
-//        1                           scout: pages and scales, some blocks ahead (and one or two warps fill up the warpgroup)
+// Warps: 4 per sub-tile  softmax, one thread per row (P, rescale of O, epilogue); each loads its rows of Q
+//        4               converters: two turn K's codes into fp16 tiles in the swizzled operand layout, two V's
+//        1 per sub-tile  MMA issue
+//        1               scout: pages and scales, some blocks ahead (and one or two warps fill up the warpgroup)
+// Two sub-tiles of 128 rows against the same keys, or (DUAL: no more than 128 rows) the same rows against even and odd key blocks, merged
+// in the epilogue: with one chain of score, softmax and product a CTA of 128 rows idles between its steps (two such CTAs an SM: 55 us for
+// drafts of 3 - 16 tokens, 8 heads a group, over 3001 - 20000 keys; DUAL 43.5).  256 columns: one sub-tile, O fills TMEM.
 // Blocks of 64 keys, two S buffers per sub-tile: S of block j + 1 is there when the softmax of block j ends, so its threads wait for no
 // product.  A thread keeps its 64 scores in registers, and P' goes back into the columns it read, as the TMEM operand of P.V: no
 // shared-memory traffic and no proxy fence for P.  S of block j + 2 lands on P of block j; the same thread issues both products, in
-// this order.  TMEM: per sub-tile S 2 x 64, O 128 columns; one sub-tile with 256 columns of O for head dims above 128.
-// (Before, 128 keys at a time, P through shared memory, S read twice from TMEM: 636 us for four chunks of 301 - 2048 tokens against
-// 1777 - 8192 keys, 32 / 8 heads, of which a third was waiting for products and fences.)
+// this order.  TMEM: per sub-tile S 2 x 64, O 128 columns.
+// TMA cannot convert, so the codes pass through registers: copied ahead into shared memory as they are, read back by the thread that asked
+// for them, turned and stored again.
 //
-// Bound: per 128 keys and 256 rows of head dim 128 the products take 2048 cycles of an SM's tensor pipe, the exponentials 2048 of its
-// special-function unit, 320 KB through shared memory 2560, turning the codes about 1000 of 8192 issue slots.  TMA cannot convert,
-// so the codes pass through registers.
+// Bound: four chunks of 301 - 2048 tokens against 1777 - 8192 keys, 32 / 8 heads of 128: 485 us, 880 TFLOP/s of what the masks leave.  Per 64
+// keys and 256 rows a CTA takes 2400 cycles; the products take 1024 of them on the tensor pipe, the exponentials 1024 on the special-function
+// unit, shared memory is busy for 750.  What is left is the chain of one softmax warp (poll, TMEM load, maximum, exponentials, TMEM store,
+// fence) with two such warps a scheduler, as many as registers allow: without any exponential it still takes 1950.  Tried and without
+// gain: a quarter of the exponentials as polynomials (485), a look at the next block's barriers ahead of time (515 - 535), blocks of 128 keys
+// with P through shared memory (636).
 #pragma once
 
 #include <type_traits>

@@ -177,7 +177,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
     (pages or cache rows, blocks of tokens, nheads_k): an element stands for code * scale of its (block, head).  Blocks have
     equal, whole multiples of 16 tokens: a page (or a cache row) divided by the second dimension.  Head dims are multiples of 16.  k / v are then
     appended as ``quantized_kvcache_append`` does -- codes and scales change in place -- and attended to as the cache
-    holds them.  scheduler_metadata and q_descale are refused."""
+    holds them.  Codes of tokens that no query of the sequence sees may be anything; a NaN code of a value that some query sees may
+    reach others whose mask hides it (their weight is 0, and 0 * NaN is NaN).  scheduler_metadata and q_descale are refused."""
     if softmax_scale is None:
         softmax_scale = _default_scale(q, qv)
     if kv8.holds_codes(k_cache, v_cache):

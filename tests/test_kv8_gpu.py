@@ -1,4 +1,5 @@
 """GPU: serving from a KV cache held in 8 bits -- step plan, quantising append, attention -- against plain forms in 64 bits."""
+import ctypes as C
 import math
 
 import pytest
@@ -6,6 +7,7 @@ import torch
 
 import flash_attn_npu_v3 as fa3
 import kv8_util as U
+from flash_b200 import kv8
 from flash_b200 import lib as L
 from flash_b200 import ops
 from kv8_util import BF, E4M3, FP, INT8
@@ -511,6 +513,134 @@ def test_streams_and_calls_at_once():
         torch.cuda.synchronize()
         for (o, l), (o1, l1) in zip(got, alone):
             assert torch.equal(o, o1) and torch.equal(l, l1)
+
+
+@pytest.mark.parametrize("s_q,h,h_k,d,dtype,codes,mask", [
+    (5, 16, 2, 64, BF, E4M3, dict(causal=True)), (16, 8, 1, 128, FP, INT8, {}), (6, 12, 2, 96, BF, INT8, dict(causal=True, window=(90, 0))),
+    (9, 8, 2, 64, FP, E4M3, dict(softcap=15.0)), (33, 4, 2, 128, BF, E4M3, dict(window=(70, 20)))])
+@pytest.mark.parametrize("b,most", [(3, 900), (110, 330)])
+def test_between_decode_and_prompt(s_q, h, h_k, d, dtype, codes, mask, b, most):
+    """33 to 128 rows of a kv head: key blocks of 64 in two streams.  Few long sequences, which CTAs share, and many short ones, several a
+    CTA: one block, an odd number, none at all, a first block that falls to either stream."""
+    g = _gen(s_q * 100 + b)
+    lens = [0, 1, 64, 65, 129, 200][:b] + torch.randint(0, most, (max(0, b - 6),), generator=g).tolist()
+    if b == 3:
+        lens = [most, 0, most // 2 + 1]
+    kc, ks, table, kv = _cache_for(g, lens, 32, 16, h_k, d, codes)
+    q = torch.randn((b, s_q, h, d), generator=g).to(dtype)
+    causal, window, cap = mask.get("causal", False), mask.get("window", (-1, -1)), mask.get("softcap", 0.0)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), kc.cuda(), cache_seqlens=_i32(lens), page_table=table.cuda(), k_descale=ks.cuda(),
+                                               v_descale=ks.cuda(), causal=causal, window_size=window, softcap=cap, return_softmax_lse=True)
+    is_causal, is_local, wl, wr = L.normalize_window(s_q, max(lens), causal, *window)
+    for r in range(b):
+        want = U.attend(q[r], kv[r], kv[r], d ** -0.5, is_causal, (wl, wr) if is_local else None, cap)
+        U.check_attention(out[r], lse[r], want, cap, f"sequence {r} of {lens[r]}")
+    _status()
+
+
+@pytest.mark.parametrize("page,sb", [(160, 32), (48, 16), (320, 160), (64, 64), (16, 16), (0, 16)])
+def test_pages_that_do_not_divide_a_stage(page, sb):
+    """32 rows of 128 columns take stages of 160 keys: boxes of a page, of a part of it, of a whole stage."""
+    g = _gen(page + 1)
+    lens = [960, 481, 160, 1]
+    kc, ks, table, kv = _cache_for(g, lens, page, sb, 2, 128, E4M3)
+    q = torch.randn((4, 4, 16, 128), generator=g).to(BF)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), kc.cuda(), cache_seqlens=_i32(lens), page_table=table.cuda() if page else None,
+                                               k_descale=ks.cuda(), v_descale=ks.cuda(), causal=True, return_softmax_lse=True)
+    for r in range(4):
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv[r], kv[r], 128 ** -0.5, True), tag=f"sequence {r}")
+    _status()
+
+
+@pytest.mark.parametrize("s_q,h,where", [(8, 16, "k"), (8, 16, "v"), (40, 16, "k"), (40, 16, "v")])
+@pytest.mark.parametrize("token", [3, 70, 299])
+def test_nan_among_many_rows(s_q, h, where, token):
+    """One NaN code, in a block of either stream: a key's reaches every row that sees it and no other; a value's the one column of every row
+    that sees it -- and of others, where its weight is 0 and 0 * NaN is NaN, as in the formula."""
+    g = _gen(token)
+    kc, ks, table, kv = _cache_for(g, [300], 32, 32, 2, 64, E4M3)
+    vc = kc.clone()
+    (kc if where == "k" else vc).view(torch.uint8)[int(table[0, token // 32]), token % 32, 0, 5] = 127
+    q = torch.randn((1, s_q, h, 64), generator=g).to(BF)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), vc.cuda(), cache_seqlens=_i32([300]), page_table=table.cuda(), causal=True,
+                                               k_descale=ks.cuda(), v_descale=ks.cuda(), return_softmax_lse=True)
+    sees = torch.arange(s_q) + 300 - s_q >= token
+    gone = out[0].isnan().cpu()
+    assert not bool(gone[:, h // 2:].any())
+    if where == "k":
+        assert not bool(gone[~sees].any()) and bool(gone[sees][:, :h // 2].all()) and bool(lse[0, :h // 2].cpu()[:, sees].isnan().all())
+    else:
+        assert bool(gone[sees][:, :h // 2, 5].all()) and int(gone.sum()) == int(gone[..., 5].sum())
+        assert bool(lse.isfinite().all())
+    rest = slice(h // 2, h)  # of the other kv head
+    U.check_attention(out[0, :, rest], lse[0, rest], U.attend(q[0, :, rest], kv[0][:, 1:], kv[0][:, 1:], 64 ** -0.5, True))
+
+
+@pytest.mark.parametrize("q_lens,h,splits", [([1, 0, 3], 8, 0), ([16, 3, 0], 16, 0), ([16, 3, 0], 16, 3), ([130, 5, 60], 8, 0), ([130, 5, 60], 8, 2)])
+def test_rows_behind_the_last_sequence(q_lens, h, splits):
+    """A padded batch: rows that belong to no sequence are left as they were, whatever is merged."""
+    g = _gen(sum(q_lens))
+    lens, d, pad = [700, 400, 90], 64, 5
+    kc, ks, table, kv = _cache_for(g, lens, 64, 32, 2, d, E4M3)
+    kc, ks, table = kc.cuda(), ks.cuda(), table.cuda()
+    n = sum(q_lens)
+    q = torch.randn((n + pad, h, d), generator=g).to(BF).cuda()
+    cu = [sum(q_lens[:i]) for i in range(4)]
+    out, lse = torch.full_like(q, 7.0), torch.full((h, n + pad), 7.0, device="cuda")
+    c = kv8._cache_block(kc, kc, ks, ks, q)
+    cu_t, lens_t = _i32(cu), _i32(lens)
+    p = ops.build_params(q, kc, kc, out, lse, cu_seqlens_q=cu_t, max_seqlen_q=max(q_lens), seqused_k=lens_t, block_table=table, softmax_scale=d ** -0.5,
+                         causal=True, window_left=-1, window_right=-1, softcap=0.0, num_splits=splits)
+    lib = L.load()
+    nbytes = lib.fa_b200_kv8_fwd_workspace(C.byref(p), C.byref(c))
+    ws = torch.full((max(nbytes, 16),), 255, dtype=torch.uint8, device="cuda")  # (NaN wherever nothing is written)
+    L.check(lib.fa_b200_kv8_fwd(C.byref(p), C.byref(c), ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream))
+    assert bool((out[n:] == 7).all()) and bool((lse[:, n:] == 7).all())
+    for r in range(3):
+        rows = slice(cu[r], cu[r + 1])
+        U.check_attention(out[rows], lse[:, rows], U.attend(q[rows].cpu(), kv[r], kv[r], d ** -0.5, True), tag=f"sequence {r}")
+
+
+def test_new_tokens_without_queries():
+    """A call with no query row still appends."""
+    g = _gen(21)
+    kc, ks, table, _ = _cache_for(g, [40, 70], 32, 32, 2, 64, E4M3)
+    x = torch.randn((2, 3, 2, 64), generator=g).to(BF).cuda()
+    table, lens = table.cuda(), _i32([37, 67])
+    slots = torch.tensor([int(table[r, t // 32]) * 32 + t % 32 for r, n in enumerate((37, 67)) for t in range(n, n + 3)], device="cuda")
+    state = [[kc.cuda(), kc.cuda(), ks.cuda(), ks.cuda()] for _ in range(2)]
+    out = fa3.flash_attn_with_kvcache(torch.empty((2, 0, 4, 64), dtype=BF, device="cuda"), *state[0][:2], x, x, cache_seqlens=lens, page_table=table,
+                                      k_descale=state[0][2], v_descale=state[0][3])
+    fa3.quantized_kvcache_append(x.flatten(0, 1), x.flatten(0, 1), *state[1], slots)
+    assert out.shape == (2, 0, 4, 64)
+    for a, b in zip(*state):
+        assert torch.equal(_raw(a), _raw(b))
+
+
+@pytest.mark.parametrize("blocks", [1, 8])
+@pytest.mark.parametrize("codes", [E4M3, INT8])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_append_of_special_values(dtype, codes, blocks):
+    """Long and short runs whose elements are infinite, NaN, zero, subnormal or halfway between codes, next to ones that are not."""
+    g = _gen(31)
+    n, d = 200, 64
+    for first in (0, 5):
+        kc, ks = _random_cache(g, 3, 128, 2, d, blocks, codes)
+        x = torch.randn((n, 2, d), generator=g) * 3
+        x[10, 0, 3], x[20, 0, 4], x[30, 0, 5] = math.inf, -math.inf, math.nan
+        x[40:60] = 0.0
+        x[60:80] *= 2.0 ** -24 if dtype == FP else 2.0 ** -130
+        x[80:100] = torch.randint(-254, 255, (20, 2, d), generator=g) / 2.0  # halves of an int8 code at scale 1
+        x = x.to(dtype)
+        want_c, want_s = kc.clone(), ks.clone()
+        slots = list(range(128 + first, 128 + first + 100)) + list(range(first, first + 100))
+        U.append(x, want_c, want_s, slots)
+        got = [kc.cuda(), kc.cuda(), ks.cuda(), ks.cuda()]
+        fa3.quantized_kvcache_append(x.cuda(), x.cuda(), *got, torch.tensor(slots, device="cuda"))
+        for c, s in (got[0::2], got[1::2]):
+            assert torch.equal(s.cpu(), want_s)
+            a, b = U.values_of(c.cpu()), U.values_of(want_c)
+            assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
 
 
 def test_under_torch_compile():

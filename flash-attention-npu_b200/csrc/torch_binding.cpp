@@ -421,20 +421,21 @@ PyObject* tuple_of(std::initializer_list<Tensor> ts) {
 }
 
 // kvcache8(q, k_cache, v_cache, k, v, cu_seqlens_q, max_seqlen_q, cache_seqlens, cache_batch_idx, page_table, rotary_cos, rotary_sin,
-//          rotary_interleaved, k_descale, v_descale, softmax_scale, causal, window_left, window_right, softcap, num_splits)
-//   -> (out, lse), or NotImplemented
+//          rotary_interleaved, k_descale, v_descale, softmax_scale, causal, window_left, window_right, softcap, num_splits, all)
+//   -> (out, lse), with `all` (out, lse, empty, empty), or NotImplemented
 PyObject* kvcache8(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   FwdArgs a;
   fa_fwd_params p;
   fa_kv8_cache c;
   const Tensor *ks, *vs;
-  if (n != 21 || !plain_eager()) return not_implemented();
+  bool all = false;
+  if (n != 22 || !plain_eager()) return not_implemented();
   if (!as_tensor(o[0], a.q) || !as_tensor(o[1], a.k) || !as_tensor(o[2], a.v) || !as_tensor(o[3], a.k_new) || !as_tensor(o[4], a.v_new) ||
       !as_tensor(o[5], a.cu_q) || (a.cu_q && !as_int(o[6], a.max_q)) || !as_tensor(o[7], a.seqused_k) || !as_tensor(o[8], a.batch_idx) ||
       !as_tensor(o[9], a.table) || !as_tensor(o[10], a.cos) || !as_tensor(o[11], a.sin) || !as_bool(o[12], a.interleaved) ||
       !as_tensor(o[13], ks) || !as_tensor(o[14], vs) || !as_float(o[15], a.scale) || !as_bool(o[16], a.causal) || !as_int(o[17], a.wl) ||
-      !as_int(o[18], a.wr) || !as_float(o[19], a.softcap) || !as_int(o[20], a.num_splits))
+      !as_int(o[18], a.wr) || !as_float(o[19], a.softcap) || !as_int(o[20], a.num_splits) || !as_bool(o[21], all))
     return not_implemented();
   if (!a.q || !fill_scales(a.k, a.v, ks, vs, c) || a.k->device() != a.q->device()) return not_implemented();
   a.kv8 = &c;
@@ -443,6 +444,10 @@ PyObject* kvcache8(PyObject*, PyObject* const* o, Py_ssize_t n) {
   Tensor out, lse;
   if (!launch_forward(a, p, out, lse)) return not_implemented();
   if (a.k_new) wrote({a.k, a.v, ks, vs});
+  if (all) {
+    const auto none = at::TensorOptions().dtype(c10::get_default_dtype_as_scalartype()).device(out.device());
+    return tuple_of({out, lse, at::empty({0}, none), at::empty({0}, none)});
+  }
   return two(std::move(out), std::move(lse));
   END_HANDLE_TH_ERRORS
 }

@@ -187,9 +187,9 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
                 and not torch.compiler.is_compiling()):
             r = _native.kvcache8(q, k_cache, v_cache, k, v, cu_seqlens_q, max_seqlen_q, cache_seqlens, cache_batch_idx, page_table,
                                  rotary_cos, rotary_sin, rotary_interleaved, k_descale, v_descale, softmax_scale, causal,
-                                 window_size[0], window_size[1], softcap, num_splits)
+                                 window_size[0], window_size[1], softcap, num_splits, return_softmax_lse)
             if r is not NotImplemented:
-                return (*r, torch.empty((0,), device=q.device), torch.empty((0,), device=q.device)) if return_softmax_lse else r[0]
+                return r if return_softmax_lse else r[0]
         out, lse = _kvcache_8bit(
             q, k_cache, v_cache, k, v, qv, rotary_cos, rotary_sin, cache_seqlens, cache_batch_idx, cache_leftpad, page_table,
             cu_seqlens_q, cu_seqlens_k_new, max_seqlen_q, rotary_seqlens, q_descale, k_descale, v_descale, softmax_scale, causal,

@@ -82,26 +82,7 @@ struct Kv8TileShared {
   int abort_flag;
 };
 
-// Bounded wait for two or three barriers at once: a poll takes some 160 cycles even where there is nothing to wait for, and three in a
-// row are a sixth of a block's softmax.
-__device__ __forceinline__ bool kv8_wait3(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2, volatile int* abort_flag, int id) {
-  for (uint32_t i = 0; i < tc5::kSpinLimit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p, q, r;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
-        "and.pred p, p, q;\n\tand.pred p, p, r;\n\tselp.b32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(b0), "r"(p0), "r"(b1), "r"(p1), "r"(b2), "r"(p2)
-        : "memory");
-    if (ok) return true;
-    if ((i & 255u) == 255u && *abort_flag) return false;
-  }
-  if (*abort_flag == 0) *abort_flag = id;
-  return false;
-}
+// Bounded wait for two barriers at once: a poll takes some 160 cycles even where there is nothing to wait for.
 __device__ __forceinline__ bool kv8_wait2(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, volatile int* abort_flag, int id) {
   for (uint32_t i = 0; i < tc5::kSpinLimit; ++i) {
     uint32_t ok;
@@ -453,10 +434,9 @@ __device__ __forceinline__ bool kv8_softmax(const Kv8Params& p, const Kv8Mask& m
     if (!Tr::mine(first + it, t)) continue;
     const int n = Tr::local(first + it), b = n & 1, e = (first + it) % Tr::SCR, t0 = (lo + it) * Tr::BN;
     const uint32_t s_tmem = tmem + t * Tr::SUB_STEP + b * Tr::BN + lane_base;
-    // (P.V of two blocks before is over when S of this one is there, but no phase of a barrier may be missed.  In front of the first two
-    // blocks there was none: the phase before a barrier's first counts as over.)
-    if (!kv8_wait3(tc5::smem_addr(&sh->s_full[t][b]), (n >> 1) & 1, tc5::smem_addr(&sh->sc_full[e]), ((first + it) / Tr::SCR) & 1,
-                   tc5::smem_addr(&sh->pv_done[t][b]), ((n >> 1) + 1) & 1, abort_flag, 79))
+    // (P.V of two blocks before is over when S of this one is there.  Where this thread waits for the one of a block, the next on that
+    // buffer cannot be over, so that a barrier is never two phases on.)
+    if (!kv8_wait2(tc5::smem_addr(&sh->s_full[t][b]), (n >> 1) & 1, tc5::smem_addr(&sh->sc_full[e]), ((first + it) / Tr::SCR) & 1, abort_flag, 79))
       return false;
     tc5::tc_fence_after();
     uint32_t r[2][32];

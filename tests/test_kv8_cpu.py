@@ -53,7 +53,8 @@ def _message(rc):
     (dict(k_scale=0), "scales"), (dict(h=12), "divide"), (dict(alibi_slopes=256), "alibi"), (dict(cu_seqlens_k=256), "cu_seqlens_k"),
     (dict(k_row_stride=1032), "16"), (dict(k=264), "16-byte"), (dict(q_row_stride=4100), "multiples of 8"),
     (dict(block_table=256, page_size=128), "kv_outer"), (dict(k_new=256, seqlen_new=1), "passed together"),
-    (dict(k_new=256, v_new=256, seqlen_new=5000), "fit"), (dict(rotary_cos=256, rotary_sin=256), "together with new"),
+    (dict(k_new=256, v_new=256, seqlen_new=5000), "fit"), (dict(k_new=256, v_new=256, seqlen_new=1 << 30, seqlen_k=1 << 30), "too many new tokens"),
+    (dict(rotary_cos=256, rotary_sin=256), "together with new"),
     (dict(k_new=256, v_new=256, seqlen_new=1, rotary_cos=256, rotary_sin=256, rotary_dim=128, rotary_seqlen=4095), "every position"),
     (dict(softcap=-1.0), "softcap"), (dict(partial_out=1), "partial"), (dict(lse_head_stride=2), "contiguous"), (dict(dtype=2), "FP16 and BF16")])
 def test_attention_refusals(change, said):
@@ -74,7 +75,7 @@ def test_workspace_holds_the_partials():
 @pytest.mark.parametrize("change,said", [
     (dict(d=24), "multiple of 16"), (dict(rows=100), "divide"), (dict(k=8), "16-byte"), (dict(k_tok_stride=100), "multiples of 8"),
     (dict(kc_row_stride=1028), "16"), (dict(dtype=5), "FP16 and BF16"), (dict(slots=0), "non-null"), (dict(total=-1), "sizes"),
-    (dict(kv_outer=0), "sizes")])
+    (dict(kv_outer=0), "sizes"), (dict(h_k=32768), "too many new tokens or heads"), (dict(kv_outer=1 << 25), "too many tokens in the KV cache")])
 def test_append_refusals(change, said):
     p = L.Kv8AppendParams()
     p.k = p.v = p.k_cache = p.v_cache = p.slots = 256

@@ -945,7 +945,7 @@ int fa_b200_check_status(void* stream) {
     return fa::fail(FA_ERR_CUDA, "a rank did not deliver its partial to the cross-GPU merge within the time limit "
                                  "(results of that call are invalid)");
   if (v & fa::kStatusBadIndex)
-    return fa::fail(FA_ERR_INVALID, "a block_table / cache_batch_idx entry or a cache length was out of range "
+    return fa::fail(FA_ERR_INVALID, "a block_table / cache_batch_idx entry, a slot, a length or an offset was out of range "
                                     "(the kernels read zeros instead; results of that launch are invalid)");
   if (v & 0x40000000)
     return fa::fail(FA_ERR_CUDA, "a bounded device-side wait gave up in CTA " + std::to_string(v & 0xffffff) +

@@ -3,7 +3,9 @@
 //
 // Request r holds ceil(have / page) pages and needs ceil((have + new) / page).  The missing ones come off the free list in request
 // order, so request r's start in the list is a prefix sum; a request whose row of the table or the list has no room is left as it
-// was (the prefix sum goes on as if it had been served, so that the pages taken are always the list's first ones).
+// was (the prefix sum goes on as if it had been served, so that the pages taken are always the list's first ones).  So is a request
+// whose tokens would end behind the packed batch's rows: it, and every one behind it that brings any.  The sums stop at INT32_MAX,
+// where they are behind any batch and any list: lengths may be anything.
 //
 // Latency-bound: a few bytes a token.  One launch: every CTA sums up all requests by itself (two prefix sums of b entries, from L2)
 // and then writes its share of the tokens and of the table, a token a thread up to a CTA for every SM, so no CTA waits for another.
@@ -34,6 +36,10 @@ __device__ __forceinline__ PlanRequest plan_request(const fa_kvcache_plan_params
 }
 __device__ __forceinline__ PlanRequest plan_request(const fa_kvcache_plan_params& p, int r) { return plan_request(p, p.have[r], p.add[r]); }
 
+// Sums of numbers that are not negative.
+__device__ __forceinline__ int capped_sum(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7fffffffu); }
+__device__ __forceinline__ int2 capped_sum(int2 a, int2 b) { return make_int2(capped_sum(a.x, b.x), capped_sum(a.y, b.y)); }
+
 __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid_constant__ fa_kvcache_plan_params p, int32_t* status) {
   extern __shared__ int2 s_pre[];  // per request: tokens and pages in front of it; [b]: of all
   __shared__ int2 s_warp[kPlanThreads / 32];
@@ -55,28 +61,31 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
       if (rb + k >= r1) break;
       const PlanRequest q = plan_request(p, have[k], add[k]);
       s_pre[rb + k] = sum;
-      sum.x += (int)q.add;
-      sum.y += q.need;
+      sum = capped_sum(sum, make_int2((int)q.add, q.need));
     }
   }
   int2 incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
-    if (lane >= o) { incl.x += x; incl.y += y; }
+    if (lane >= o) incl = capped_sum(incl, make_int2(x, y));
   }
   if (lane == 31) s_warp[warp] = incl;
   if (tid == 0) s_pages = 0;
   __syncthreads();
-  int2 base = make_int2(incl.x - sum.x, incl.y - sum.y);
-  for (int w = 0; w < warp; ++w) { base.x += s_warp[w].x; base.y += s_warp[w].y; }
-  for (int r = r0; r < r1; ++r) { s_pre[r].x += base.x; s_pre[r].y += base.y; }
-  if (tid == kPlanThreads - 1) s_pre[p.b] = make_int2(base.x + sum.x, base.y + sum.y);
+  int2 base = make_int2(__shfl_up_sync(0xffffffffu, incl.x, 1), __shfl_up_sync(0xffffffffu, incl.y, 1));
+  if (lane == 0) base = make_int2(0, 0);
+  for (int w = 0; w < warp; ++w) base = capped_sum(base, s_warp[w]);
+  for (int r = r0; r < r1; ++r) s_pre[r] = capped_sum(s_pre[r], base);
+  if (tid == kPlanThreads - 1) s_pre[p.b] = capped_sum(base, sum);
   __syncthreads();
 
   int n_free = p.n_free;
   if (p.num_free) n_free = min(max(*p.num_free, 0), p.n_free);
-  auto granted = [&](const PlanRequest& q, int r) { return q.fits && (q.need == 0 || s_pre[r].y + q.need <= n_free); };
+  auto behind = [&](const PlanRequest& q, int r) { return q.add > 0 && s_pre[r].x + q.add > p.total; };  // of the packed batch's rows
+  auto granted = [&](const PlanRequest& q, int r) {
+    return q.fits && !behind(q, r) && (q.need == 0 || (int64_t)s_pre[r].y + q.need <= n_free);
+  };
   // requests: a warp each
   const int warps = gridDim.x * (kPlanThreads / 32), gw = blockIdx.x * (kPlanThreads / 32) + warp;
   for (int r = gw; r < p.b; r += warps) {
@@ -84,8 +93,8 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
     const bool ok = granted(q, r);
     if (lane == 0) {
       p.after[r] = (int)(ok ? q.have + q.add : p.have[r]);
-      p.cu_new[r] = s_pre[r].x;
-      if (!ok && !(q.have >= 0 && p.add[r] >= 0)) raise_bad_index(status);
+      p.cu_new[r] = (int)min((int64_t)s_pre[r].x, p.total);
+      if (q.have < 0 || p.add[r] < 0 || behind(q, r)) raise_bad_index(status);
     }
     if (ok)
       for (int i = lane; i < q.need; i += 32) p.table[(int64_t)r * p.table_stride + q.had + i] = p.free_pages[s_pre[r].y + i];
@@ -100,7 +109,7 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
     __syncthreads();
     if (tid == 0) {
       *p.pages_taken = s_pages;
-      p.cu_new[p.b] = s_pre[p.b].x;
+      p.cu_new[p.b] = (int)min((int64_t)s_pre[p.b].x, p.total);
     }
   }
   // tokens

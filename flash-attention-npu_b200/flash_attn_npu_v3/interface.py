@@ -295,7 +295,8 @@ def paged_kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_
     free_pages (int32; its first num_free[0] entries where num_free, an int32 tensor of one element, is given) in request
     order and written into its row of page_table (batch, max_pages) int32, in place.  A request that its row or the free list
     has no room for is left as it was.  total_new: rows of the packed batch, the sum of new_seqlens or more (the rows behind
-    are padding).  Up to 16384 requests.
+    are padding); requests whose tokens would end behind it are left as they were too, and the device's status word
+    (fa_b200_check_status) tells of them, as of negative lengths.  Up to 16384 requests.
 
     Returns (slot_mapping (total_new,) int64: where ``quantized_kvcache_append`` puts each packed token, -1 for padding and
     requests left out; cu_seqlens (batch + 1,) int32 offsets of the requests in the packed batch; cache_seqlens afterwards

@@ -328,10 +328,11 @@ int fa_b200_kv8_append(const fa_kv8_append_params* p, void* stream);
 
 /* One serving step's bookkeeping from the requests' lengths, on the device.  Request r holds have[r] tokens in ceil(have / page_size)
  * pages named by its row of the table and brings add[r] more; the pages it lacks are taken off free_pages in request order and written into
- * its row.  A request that its row or the free list has no room for stays as it was.  Outputs: cu_new (b + 1) offsets of the
+ * its row.  A request that its row or the free list has no room for, or whose tokens would end behind the packed batch, stays as it was.  Outputs: cu_new (b + 1) offsets of the
  * requests' new tokens in the packed batch; after (b) lengths afterwards; slots (total): page * page_size + row of each packed
  * token, -1 for tokens of a refused request and rows behind the last one; positions (total) in their sequence, 0 behind the last;
- * pages_taken (1).  Negative lengths are refused like that and reported by fa_b200_check_status. */
+ * pages_taken (1).  Negative lengths are refused like that; they and tokens behind the packed batch are reported by fa_b200_check_status, and
+ * no offset is above total. */
 #define FA_B200_PLAN_MAX_REQUESTS 16384
 typedef struct fa_kvcache_plan_params {
   const int32_t* have;

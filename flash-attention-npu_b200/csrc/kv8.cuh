@@ -8,6 +8,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "kv8_ranges.cuh"
 #include "tc5_ptx.cuh"
 
 namespace fa {
@@ -87,8 +88,15 @@ __device__ __forceinline__ void kv8_key_range(const Kv8Mask& m, int k_len, int k
   if (hi < lo) hi = lo;
 }
 
-__device__ __forceinline__ int kv8_q_len(const Kv8Params& p, int bi) {
-  return p.a.cu_seqlens_q ? p.a.cu_seqlens_q[bi + 1] - p.a.cu_seqlens_q[bi] : p.a.seqlen_q;
+// Query rows of a sequence.  Offsets out of range are cut to the rows there are; runs longer than the caller said, of which the tiles cover
+// no more than that, are reported like them.
+__device__ __forceinline__ void kv8_q_rows(const Kv8Params& p, int bi, int& row0, int& len) {
+  row0 = 0;
+  len = p.a.seqlen_q;
+  if (p.a.cu_seqlens_q) {
+    const bool fine = kv8_query_rows(p.a.cu_seqlens_q[bi], p.a.cu_seqlens_q[bi + 1], p.a.total_q, row0, len);
+    if (!fine || len > p.a.seqlen_q) raise_bad_index(p.status);
+  }
 }
 __device__ __forceinline__ int kv8_k_len(const Kv8Params& p, int bi) {
   return (p.a.seqused_k ? cache_len(p.a, bi, p.status) : p.a.seqlen_k) + p.a.seqlen_new;
@@ -97,8 +105,7 @@ __device__ __forceinline__ int kv8_k_len(const Kv8Params& p, int bi) {
 // block_m: rows of a tile
 __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Params& p, const Kv8Mask& m, int bi, int mb, int block_m) {
   Kv8Seq s;
-  s.q_row0 = p.a.cu_seqlens_q ? p.a.cu_seqlens_q[bi] : 0;
-  s.q_len = kv8_q_len(p, bi);
+  kv8_q_rows(p, bi, s.q_row0, s.q_len);
   s.k_len = kv8_k_len(p, bi);
   s.koff = s.k_len - s.q_len;
   const int i_lo = mb * block_m / p.group, i_hi = min(s.q_len, (mb * block_m + block_m - 1) / p.group + 1) - 1;
@@ -131,7 +138,9 @@ struct Kv8Walk {
   int bi, nb_lo, nb_hi, n_b, quota, cur, g1, ustart;
 
   __device__ __forceinline__ static void blocks(const Kv8Params& p, const Kv8Mask& m, int bi, int mb, int& nb_lo, int& nb_hi) {
-    const int q_len = kv8_q_len(p, bi), k_len = kv8_k_len(p, bi);
+    int q_row0, q_len;
+    kv8_q_rows(p, bi, q_row0, q_len);
+    const int k_len = kv8_k_len(p, bi);
     const int i_lo = mb * BM / p.group, i_hi = min(q_len, (mb * BM + BM - 1) / p.group + 1) - 1;
     int lo, hi;
     kv8_key_range(m, k_len, k_len - q_len, i_lo, i_hi, lo, hi);

@@ -295,6 +295,7 @@ typedef struct fa_kv8_cache {
 /* fa_b200_fwd over such a cache: p->k / p->v are codes (strides in elements), p->dtype is the type of q, o, k_new and v_new.
  * Dense or packed (cu_seqlens_q) queries; contiguous (cache_batch_idx) or paged caches; causal, window, softcap, rotary
  * with k_new.  New tokens are appended as fa_b200_kv8_append does and then attended to as the cache holds them.
+ * Offsets (cu_seqlens_q) beyond the total_q rows are cut to them, and reported by fa_b200_check_status as are runs longer than seqlen_q.
  * Not here: cu_seqlens_k, alibi, sharded positions, partial_out.  num_splits as in fa_b200_fwd; p->kernel is not read. */
 int fa_b200_kv8_fwd(const fa_fwd_params* p, const fa_kv8_cache* c, void* workspace, size_t workspace_bytes, void* stream);
 size_t fa_b200_kv8_fwd_workspace(const fa_fwd_params* p, const fa_kv8_cache* c); /* 0 also for a call that would be refused */

@@ -1,0 +1,64 @@
+"""CPU: refusals at the edges of the contract of the operators around an 8-bit KV cache, and the index arithmetic that keeps their kernels
+within their tensors.  Nothing is launched."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+import flash_attn_npu_v3 as fa3
+from flash_b200 import kv8
+from flash_b200 import lib as L
+from test_kv8_cpu import _fwd, _message
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flash-attention-npu_b200", "csrc")
+
+
+RANDOM = r"""
+#include <cstdio>
+#include <initializer_list>
+#include <limits>
+#include <random>
+#include "kv8_ranges.cuh"
+std::mt19937 rng(5);
+int any() {
+  const int top = std::numeric_limits<int>::max(), low = std::numeric_limits<int>::min();
+  switch (rng() % 6) {
+    case 0: return 0;
+    case 1: return top - (int)(rng() % 3);
+    case 2: return low + (int)(rng() % 3);
+    case 3: return (int)(rng() % 200);
+    case 4: return -(int)(rng() % 200);
+    default: return (int)rng();
+  }
+}
+int some() { return any() & std::numeric_limits<int>::max(); }
+"""
+
+
+def _run(tmp_path, source):
+    src, exe = tmp_path / "ranges.cpp", tmp_path / "ranges"
+    src.write_text(RANDOM + source)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", CSRC, str(src), "-o", str(exe)], check=True)
+    subprocess.run([str(exe)], check=True)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no host compiler")
+def test_query_rows_are_among_the_rows_there_are(tmp_path):
+    """Whatever the offsets hold; and as given wherever that is possible."""
+    _run(tmp_path, r"""
+int main() {
+  for (int round = 0; round < 400000; ++round) {
+    const int total = round % 3 ? (int)(rng() % 100) : some(), from = any(), upto = any();
+    int row0, len;
+    const bool as_given = fa::kv8_query_rows(from, upto, total, row0, len), fine = from >= 0 && upto >= from && upto <= total;
+    if (row0 < 0 || len < 0 || (long long)row0 + len > total || as_given != fine || (fine && (row0 != from || len != upto - from))) {
+      std::printf("rows %d %d of %d: %d %d %d\n", from, upto, total, row0, len, (int)as_given);
+      return 1;
+    }
+  }
+  return 0;
+}
+""")

@@ -1,5 +1,6 @@
 """GPU: what the operators around an 8-bit KV cache do at the edges of their contract -- indices and lengths out of range, more tokens than rows,
 numbers of every size in both attention kernels, negative softmax scales, windows as long as the longest sequence."""
+import ctypes as C
 import math
 
 import pytest
@@ -7,7 +8,9 @@ import torch
 
 import flash_attn_npu_v3 as fa3
 import kv8_util as U
+from flash_b200 import kv8
 from flash_b200 import lib as L
+from flash_b200 import ops
 from kv8_util import BF, E4M3, FP, INT8
 from test_kv8_gpu import _cache_for, _gen, _i32, _random_cache, _raw, _status
 
@@ -55,3 +58,38 @@ def test_plan_of_negative_lengths(have, new):
     assert after.tolist() == [have[0], 6] and taken.tolist() == [1] and table.tolist() == [[7, 7, 7], [7, 9, 7]]
     at = max(new[0], 0)
     assert cu.tolist() == [0, at, at + 2] and slots.tolist() == ([-1] * at + [36, 37] + [-1] * 6)[:6]
+
+
+@pytest.mark.parametrize("cu,most,rows", [
+    ([0, 3, 50], 4, [(0, 3), (3, 10)]), ([0, 3, 2 ** 31 - 1], 7, [(0, 3), (3, 10)]), ([-4, 3, 10], 7, [(0, 3), (3, 10)]),
+    ([0, 7, 2], 40, [(0, 7), (7, 7)]), ([20, 30, 10], 4, [(10, 10), (10, 10)]), ([0, 300, 10], 200, [(0, 10), (10, 10)])])
+@pytest.mark.parametrize("splits", [0, 3])
+def test_offsets_out_of_range(cu, most, rows, splits):
+    """Offsets of packed queries beyond the rows there are: the rows of the sequence end where the queries do, nothing behind them is touched, and the
+    call is reported.  Sequences whose run is longer than the longest that the caller gave have just that many rows computed."""
+    g = _gen(51)
+    lens, total, pad, h, d = [300, 120], 10, 64, 8, 64
+    kc, ks, table, kv = _cache_for(g, lens, 64, 32, 2, d, E4M3)
+    kc, ks, table = kc.cuda(), ks.cuda(), table.cuda()
+    big = torch.full((total + 2 * pad, h, d), math.nan, dtype=BF, device="cuda")  # rows in front of and behind the queries
+    q = big[pad:pad + total]
+    q.copy_(torch.randn((total, h, d), generator=g))
+    o_big, l_big = torch.full_like(big, 7.0), torch.full((pad + h * total + pad,), 7.0, device="cuda")
+    out, lse = o_big[pad:pad + total], l_big[pad:pad + h * total].view(h, total)
+    c = kv8._cache_block(kc, kc, ks, ks, q)
+    cu_t, lens_t = _i32(cu), _i32(lens)
+    p = ops.build_params(q, kc, kc, out, lse, cu_seqlens_q=cu_t, max_seqlen_q=most, seqused_k=lens_t, block_table=table, softmax_scale=0.125,
+                         causal=True, num_splits=splits)
+    lib = L.load()
+    nbytes = lib.fa_b200_kv8_fwd_workspace(C.byref(p), C.byref(c))
+    ws = torch.full((max(nbytes, 16) + 256,), 255, dtype=torch.uint8, device="cuda")
+    L.check(lib.fa_b200_kv8_fwd(C.byref(p), C.byref(c), ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream))
+    assert _reported()
+    for t in (o_big[:pad], o_big[pad + total:], l_big[:pad], l_big[pad + h * total:]):
+        assert bool((t == 7).all())
+    assert bool((ws[nbytes:] == 255).all())
+    for r, (a, b) in enumerate(rows):
+        if b > a and b - a <= most:
+            upto = min(b, cu[-1]) - a  # (rows behind the last offset belong to no sequence)
+            want = U.attend(q[a:b].cpu(), kv[r], kv[r], 0.125, True)
+            U.check_attention(out[a:a + upto], lse[:, a:a + upto], (want[0][:upto], want[1][:, :upto], want[2][:upto]), tag=f"sequence {r}")

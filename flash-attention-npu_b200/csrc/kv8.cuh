@@ -56,11 +56,6 @@ struct Kv8Seq {
   const int32_t* pages;            // paged cache
 };
 
-struct Kv8Mask {
-  int wl, wr;
-  bool causal, local;
-};
-
 // The left-window rule needs the longest sequence; warp-collective.
 __device__ __forceinline__ Kv8Mask kv8_mask(const Kv8Params& p, int lane) {
   Kv8Mask m{p.wl, p.wr, false, false};
@@ -74,18 +69,6 @@ __device__ __forceinline__ Kv8Mask kv8_mask(const Kv8Params& p, int lane) {
   m.causal = m.wl < 0 && m.wr == 0;
   m.local = (m.wl >= 0 || m.wr >= 0) && !m.causal;
   return m;
-}
-
-// Keys that the query tokens i_lo .. i_hi of a sequence see.
-__device__ __forceinline__ void kv8_key_range(const Kv8Mask& m, int k_len, int koff, int i_lo, int i_hi, int& lo, int& hi) {
-  lo = 0;
-  hi = k_len;
-  if (m.causal) hi = min(k_len, i_hi + koff + 1);
-  if (m.local) {
-    hi = min(k_len, i_hi + koff + m.wr + 1);
-    lo = max(0, i_lo + koff - m.wl);
-  }
-  if (hi < lo) hi = lo;
 }
 
 // Query rows of a sequence.  Offsets out of range are cut to the rows there are; runs longer than the caller said, of which the tiles cover

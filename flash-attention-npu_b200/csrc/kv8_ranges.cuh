@@ -20,4 +20,23 @@ FA_KV8_HD bool kv8_query_rows(int from, int upto, int total, int& row0, int& len
   return row0 == from && end == upto;
 }
 
+struct Kv8Mask {
+  int wl, wr;  // taken literally where `local`: a side below -1 ends in front of (or starts behind) the diagonal
+  bool causal, local;
+};
+
+// Keys [lo, hi) of the k_len that the query tokens i_lo .. i_hi of a sequence see; none: an empty range within them.  (A range behind
+// the last key had the page table read there, and the scales of blocks that nobody has written.)
+FA_KV8_HD void kv8_key_range(const Kv8Mask& m, int k_len, int koff, int i_lo, int i_hi, int& lo, int& hi) {
+  lo = 0;
+  hi = k_len;
+  if (m.causal && i_hi + koff + 1 < hi) hi = i_hi + koff + 1;
+  if (m.local) {
+    const int64_t first = (int64_t)i_lo + koff - m.wl, behind = (int64_t)i_hi + koff + m.wr + 1;
+    lo = first < 0 ? 0 : first > k_len ? k_len : (int)first;
+    hi = behind > k_len ? k_len : behind < lo ? lo : (int)behind;
+  }
+  if (hi < lo) hi = lo;
+}
+
 }  // namespace fa

@@ -62,3 +62,38 @@ int main() {
   return 0;
 }
 """)
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="no host compiler")
+def test_visible_keys_are_among_the_keys_there_are(tmp_path):
+    """Whatever the window; and every key that a row sees is among them, counted one by one."""
+    _run(tmp_path, r"""
+int main() {
+  for (int round = 0; round < 400000; ++round) {
+    const bool wild = round % 2;
+    const int k_len = wild ? some() / 2 : (int)(rng() % 40), q_len = wild ? 1 + some() / 4 : 1 + (int)(rng() % 12);
+    fa::Kv8Mask m{};
+    const int kind = (int)(rng() % 3);
+    m.causal = kind == 1;
+    m.local = kind == 2;
+    m.wl = wild ? any() : (int)(rng() % 24) - 6;
+    m.wr = m.causal ? 0 : wild ? any() : (int)(rng() % 24) - 6;
+    const int i_lo = (int)(rng() % q_len), i_hi = i_lo + (int)(rng() % (q_len - i_lo)), koff = k_len - q_len;
+    int lo, hi;
+    fa::kv8_key_range(m, k_len, koff, i_lo, i_hi, lo, hi);
+    if (lo < 0 || hi < lo || hi > k_len) {
+      std::printf("keys %d, rows %d, window %d %d: [%d, %d)\n", k_len, q_len, m.wl, m.wr, lo, hi);
+      return 1;
+    }
+    for (int i = i_lo; !wild && i <= i_hi; ++i)
+      for (int j = 0; j < k_len; ++j) {
+        const bool seen = m.causal ? j <= i + koff : m.local ? j >= i + koff - m.wl && j <= i + koff + m.wr : true;
+        if (seen && (j < lo || j >= hi)) {
+          std::printf("keys %d, rows %d, window %d %d: row %d key %d outside [%d, %d)\n", k_len, q_len, m.wl, m.wr, i, j, lo, hi);
+          return 1;
+        }
+      }
+  }
+  return 0;
+}
+""")

@@ -93,3 +93,22 @@ def test_offsets_out_of_range(cu, most, rows, splits):
             upto = min(b, cu[-1]) - a  # (rows behind the last offset belong to no sequence)
             want = U.attend(q[a:b].cpu(), kv[r], kv[r], 0.125, True)
             U.check_attention(out[a:a + upto], lse[:, a:a + upto], (want[0][:upto], want[1][:, :upto], want[2][:upto]), tag=f"sequence {r}")
+
+
+@pytest.mark.parametrize("s_q,h", [(1, 4), (7, 8), (20, 8), (150, 4)])
+@pytest.mark.parametrize("left,right", [(299, -1), (300, -1), (298, -1), (298, 0), (299, 0), (-5, 3), (-3, 3), (-40, 3), (2, -2)])
+def test_windows_about_the_longest_sequence(s_q, h, left, right):
+    """A left side that reaches over the longest sequence is none, also where only the device knows its length; sides below -1 are taken literally."""
+    g = _gen(47)
+    lens = [64, 300, 150]
+    kc, ks, table, kv = _cache_for(g, lens, 64, 32, 2, 64, E4M3)
+    q = torch.randn((3, s_q, h, 64), generator=g).to(BF)
+    table = torch.cat([table, torch.zeros((3, 9), dtype=torch.int32)], 1)
+    for r, n in enumerate(lens):
+        table[r, -(-n // 64):] = 2 ** 30  # (room beyond the lengths, whose pages nobody may look up)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), kc.cuda(), cache_seqlens=_i32(lens), page_table=table.cuda(), k_descale=ks.cuda(),
+                                               v_descale=ks.cuda(), window_size=(left, right), return_softmax_lse=True)
+    is_causal, is_local, wl, wr = L.normalize_window(s_q, max(lens), False, left, right)
+    for r in range(3):
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv[r], kv[r], 0.125, is_causal, (wl, wr) if is_local else None), tag=f"sequence {r}")
+    _status()

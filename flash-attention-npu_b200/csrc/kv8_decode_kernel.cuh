@@ -117,14 +117,17 @@ __device__ __forceinline__ bool kv8_producer(const Kv8Params& p, const Kv8Seq& s
     const int kv = lane / Tr::GROUPS, grp = lane % Tr::GROUPS, tg = t0 + grp * kScaleGranule;
     if (lane < 2 * Tr::GROUPS && tg < sq.key_hi && tg + kScaleGranule > sq.key_lo) {
       int o = sq.batch_row, r = tg;
+      bool there = true;
       if (sq.pages) {
-        const int pg = tg / p.a.page_size;
+        const int pg = tg / p.a.page_size, id = __ldg(sq.pages + pg);
         r = tg - pg * p.a.page_size;
-        o = outer_index(p.a, __ldg(sq.pages + pg), p.status);
+        o = outer_index(p.a, id, p.status);
+        there = o == id;  // else its codes arrive as zeros, and the scale of another page is none of theirs
       }
       const int blk = r / p.c.scale_block;
-      src = kv == 0 ? p.c.k_scale + o * p.c.ks_outer_stride + blk * p.c.ks_block_stride + sg.hk * p.c.ks_head_stride
-                    : p.c.v_scale + o * p.c.vs_outer_stride + blk * p.c.vs_block_stride + sg.hk * p.c.vs_head_stride;
+      if (there)
+        src = kv == 0 ? p.c.k_scale + o * p.c.ks_outer_stride + blk * p.c.ks_block_stride + sg.hk * p.c.ks_head_stride
+                      : p.c.v_scale + o * p.c.vs_outer_stride + blk * p.c.vs_block_stride + sg.hk * p.c.vs_head_stride;
     }
     if (git >= (uint32_t)Tr::ST && !tc5::mbar_wait(empty0 + stage * 8, ((git / Tr::ST) - 1) & 1, abort_flag)) return false;
     const uint32_t k_base = pipe + stage * Tr::STAGE_BYTES, v_base = k_base + Tr::KV_BYTES, full = full0 + stage * 8;

@@ -25,6 +25,17 @@ def _reported():
     return rc != 0
 
 
+def _values(table, page, n, codes, scale, gone=()):
+    """64-bit values of a sequence's first n tokens; pages in `gone` hold nothing (zeros)."""
+    sb = page // scale.shape[1]
+    rows = []
+    for t in range(n):
+        o, i = int(table[t // page]), t % page
+        rows.append(torch.zeros(codes.shape[2:], dtype=torch.float64) if t // page in gone else
+                    U.values_of(codes[o, i]) * scale[o, i // sb].double()[:, None])
+    return torch.stack(rows)
+
+
 # ---------------------------------------------------------------- plan
 @pytest.mark.parametrize("have,new,total,after,cu,real", [
     ([5, 0, 16], [4, 10, 3], 12, [9, 0, 16], [0, 4, 12, 12], 4),             # the second is cut, the third has no row at all
@@ -58,6 +69,79 @@ def test_plan_of_negative_lengths(have, new):
     assert after.tolist() == [have[0], 6] and taken.tolist() == [1] and table.tolist() == [[7, 7, 7], [7, 9, 7]]
     at = max(new[0], 0)
     assert cu.tolist() == [0, at, at + 2] and slots.tolist() == ([-1] * at + [36, 37] + [-1] * 6)[:6]
+
+
+# ---------------------------------------------------------------- append
+def test_append_to_slots_that_are_not_there():
+    """Slots at and behind the cache's end are skipped and reported; what is around stays as it was."""
+    g = _gen(41)
+    kc, ks = _random_cache(g, 3, 32, 2, 64, 2, E4M3)
+    x = torch.randn((6, 2, 64), generator=g).to(BF)
+    slots = [95, 96, 97, 2 ** 40, 10, 2 ** 63 - 1]
+    got = [kc.cuda(), kc.cuda(), ks.cuda(), ks.cuda()]
+    fa3.quantized_kvcache_append(x.cuda(), x.cuda(), *got, torch.tensor(slots, device="cuda"))
+    assert _reported()
+    U.append(x, kc, ks, [s if s < 96 else -1 for s in slots])
+    for c, s in (got[0::2], got[1::2]):
+        assert torch.equal(s.cpu(), ks) and torch.equal(U.values_of(c.cpu()), U.values_of(kc))
+
+
+@pytest.mark.parametrize("s_q", [2, 40])
+@pytest.mark.parametrize("bad", [6, -1, 2 ** 30, -2 ** 31])
+def test_new_tokens_on_pages_that_are_not_there(bad, s_q):
+    """A sequence whose last page's number is out of range: nothing is written for it, the others get theirs."""
+    g = _gen(42)
+    kc, ks = _random_cache(g, 6, 32, 2, 64, 2, E4M3)
+    table = torch.tensor([[0, 1], [2, bad], [4, 5]], dtype=torch.int32)
+    lens = [30, 33, 40]
+    x = torch.randn((3, 3, 2, 64), generator=g).to(BF)
+    q = torch.randn((3, s_q, 4, 64), generator=g).to(BF)
+    got = [kc.cuda(), kc.cuda(), ks.cuda(), ks.cuda()]
+    scale = 2.0 ** -14  # (the codes are any)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), *got[:2], x.cuda(), x.cuda(), cache_seqlens=_i32(lens), page_table=table.cuda(),
+                                               k_descale=got[2], v_descale=got[3], softmax_scale=scale, causal=True, return_softmax_lse=True)
+    assert _reported()
+    for r in (0, 2):
+        U.append(x[r], kc, ks, [int(table[r, t // 32]) * 32 + t % 32 for t in range(lens[r], lens[r] + 3)])
+    for c, s in (got[0::2], got[1::2]):
+        assert torch.equal(s.cpu(), ks) and torch.equal(U.values_of(c.cpu()), U.values_of(kc))
+    for r in range(3):
+        kv = _values(table[r], 32, lens[r] + 3, kc, ks, (1,) if r == 1 else ())
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv, kv, scale, True), tag=f"sequence {r}")
+
+
+# ---------------------------------------------------------------- attention
+@pytest.mark.parametrize("s_q", [1, 12, 40, 200])
+@pytest.mark.parametrize("bad", [9, -1])
+def test_a_page_that_is_not_there_holds_nothing(bad, s_q):
+    """Its keys and values are zeros, whatever stands on the page that the number would be clamped to."""
+    g = _gen(43)
+    code = torch.randint(0, 100, (9, 32, 2, 64), generator=g, dtype=torch.uint8)
+    code[0], code[8] = 127, 127
+    scale = torch.exp2(torch.randint(-3, 2, (9, 2, 2), generator=g).float())
+    scale[0], scale[8] = math.nan, math.nan
+    table = torch.tensor([[1, 2, 3, bad, 4, 5, 6], [7, 3, 5, 1, 2, 6, 4]], dtype=torch.int32)
+    q = torch.randn((2, s_q, 4, 64), generator=g).to(BF)
+    kd, sd = code.view(E4M3).cuda(), scale.cuda()
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kd, kd, cache_seqlens=_i32([200, 130]), page_table=table.cuda(), k_descale=sd, v_descale=sd,
+                                               softmax_scale=2.0 ** -12, return_softmax_lse=True)
+    assert _reported()
+    for r, n in enumerate([200, 130]):
+        kv = _values(table[r], 32, n, code.view(E4M3), scale, (3,) if r == 0 else ())
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv, kv, 2.0 ** -12), tag=f"sequence {r}")
+
+
+@pytest.mark.parametrize("s_q", [1, 40, 200])
+def test_lengths_out_of_range(s_q):
+    """A length beyond the cache counts as all of it, a negative one as none; both are reported."""
+    g = _gen(44)
+    kc, ks, table, kv = _cache_for(g, [96, 96, 96], 32, 16, 2, 64, INT8)
+    q = torch.randn((3, s_q, 4, 64), generator=g).to(FP)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), kc.cuda(), cache_seqlens=_i32([97, -3, 2 ** 31 - 1]), page_table=table.cuda(),
+                                               k_descale=ks.cuda(), v_descale=ks.cuda(), causal=True, return_softmax_lse=True)
+    assert _reported()
+    for r, n in enumerate([96, 0, 96]):
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv[r][:n], kv[r][:n], 0.125, True), tag=f"sequence {r}")
 
 
 @pytest.mark.parametrize("cu,most,rows", [

@@ -242,9 +242,10 @@ static int run_kv8_append(const fa_kv8_append_params& p_in, cudaStream_t st) {
   auto ok8 = [](int64_t s) { return s % 8 == 0; };
   if (!al16(p.k) || !al16(p.v) || !ok8(p.k_tok_stride) || !ok8(p.k_head_stride) || !ok8(p.v_tok_stride) || !ok8(p.v_head_stride))
     return fail(FA_ERR_UNSUPPORTED, "the new k, v must start at 16-byte boundaries, with strides that are multiples of 8");
-  if (p.kv_outer == 1) p.kc_outer_stride = p.vc_outer_stride = 0;
-  if (!al16(p.k_cache) || !al16(p.v_cache) || !ok8(p.kc_outer_stride) || !ok8(p.kc_row_stride) || !ok8(p.kc_head_stride) ||
-      !ok8(p.vc_outer_stride) || !ok8(p.vc_row_stride) || !ok8(p.vc_head_stride))
+  if (p.kv_outer == 1) p.kc_outer_stride = (int64_t)p.rows * p.kc_row_stride, p.vc_outer_stride = (int64_t)p.rows * p.vc_row_stride;
+  auto ok16 = [](int64_t s) { return s > 0 && s % 16 == 0; };
+  if (!al16(p.k_cache) || !al16(p.v_cache) || !ok16(p.kc_outer_stride) || !ok16(p.kc_row_stride) || !ok16(p.kc_head_stride) ||
+      !ok16(p.vc_outer_stride) || !ok16(p.vc_row_stride) || !ok16(p.vc_head_stride))
     return fail(FA_ERR_UNSUPPORTED, "the codes of an 8-bit KV cache must start at 16-byte boundaries, with strides that are multiples of 16");
   if (p.total > 0x7fffffffLL || p.h_k > 32767) return fail(FA_ERR_UNSUPPORTED, "too many new tokens or heads in one call");
   if ((int64_t)p.kv_outer * p.rows > 0x7fffffffLL) return fail(FA_ERR_UNSUPPORTED, "too many tokens in the KV cache");

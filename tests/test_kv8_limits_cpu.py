@@ -16,6 +16,49 @@ from test_kv8_cpu import _fwd, _message
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flash-attention-npu_b200", "csrc")
 
 
+def _append(**change):
+    """A call that nothing is wrong with (K and V, codes and scales in memory of their own), but for the changes."""
+    p = L.Kv8AppendParams()
+    p.k = p.v = p.slots = 256
+    p.k_cache, p.v_cache = 1 << 20, 2 << 20
+    p.k_tok_stride = p.v_tok_stride = 1024
+    p.k_head_stride = p.v_head_stride = 128
+    p.kc_outer_stride = p.vc_outer_stride = 128 * 1024
+    p.kc_row_stride = p.vc_row_stride = 1024
+    p.kc_head_stride = p.vc_head_stride = 128
+    p.total, p.kv_outer, p.rows, p.h_k, p.d, p.dtype, p.num_sm = 10, 4, 128, 8, 128, L.FA_BF16, 148
+    c = L.Kv8Cache()
+    c.k_scale, c.v_scale = 3 << 20, 4 << 20
+    c.ks_outer_stride = c.vs_outer_stride = 16
+    c.ks_block_stride = c.vs_block_stride = 8
+    c.ks_head_stride = c.vs_head_stride = 1
+    c.scale_block, c.code = 64, L.CODE_E4M3
+    for k, v in change.items():
+        setattr(c if hasattr(c, k) else p, k, v)
+    p.c = c
+    return p
+
+
+@pytest.mark.parametrize("change", [dict(kc_outer_stride=0), dict(kc_row_stride=0), dict(vc_head_stride=0), dict(vc_row_stride=1032),
+                                    dict(kc_head_stride=136), dict(kc_outer_stride=128 * 1024 + 8)])
+def test_append_takes_the_strides_that_its_header_says(change):
+    p = _append(**change)
+    assert "multiples of 16" in _message(L.load().fa_b200_kv8_append(C.byref(p), None))
+
+
+def _no_device(rc):
+    """Every check has passed: what is missing is the GPU (this test launches nothing where there is one)."""
+    return "device" in _message(rc)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would launch")
+@pytest.mark.parametrize("change", [
+    {}, dict(h_k=1, ks_head_stride=0, vs_head_stride=0, kc_head_stride=0), dict(kv_outer=1, ks_outer_stride=0, kc_outer_stride=0, vc_outer_stride=0),
+    dict(scale_block=128, ks_block_stride=0, vs_block_stride=0)])
+def test_append_strides_of_one_element_may_be_anything(change):
+    assert _no_device(L.load().fa_b200_kv8_append(C.byref(_append(**change)), None))
+
+
 RANDOM = r"""
 #include <cstdio>
 #include <initializer_list>

@@ -34,6 +34,18 @@ static int check_cache(const fa_kv8_cache& c, int rows, int d) {
   return FA_OK;
 }
 
+// New tokens are written by many warps at once, each its block and head: scales that several of them share (expanded tensors), or that K and V
+// share, would be read and written at the same time.  Reading such a cache is fine.
+static int check_written(const fa_kv8_cache& c, const void* k, const void* v, int64_t outer, int rows, int h_k) {
+  auto shared = [&](int64_t by_outer, int64_t by_block, int64_t by_head) {
+    return (outer > 1 && by_outer == 0) || (rows > c.scale_block && by_block == 0) || (h_k > 1 && by_head == 0);
+  };
+  if (k == v || c.k_scale == c.v_scale || shared(c.ks_outer_stride, c.ks_block_stride, c.ks_head_stride) ||
+      shared(c.vs_outer_stride, c.vs_block_stride, c.vs_head_stride))
+    return fail(FA_ERR_INVALID, "new tokens need a KV cache in which each of K, V and the scales has memory of its own");
+  return FA_OK;
+}
+
 struct Kv8Plan {
   Kv8Params p;
   Kv8TileInfo tile;
@@ -87,6 +99,9 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
       !ok8(a.knew_row_stride) || !ok8(a.knew_head_stride) || !ok8(a.knew_batch_stride) || !ok8(a.vnew_row_stride) ||
       !ok8(a.vnew_head_stride) || !ok8(a.vnew_batch_stride) || !al16(a.o) || !ok8(a.o_row_stride) || !ok8(a.o_head_stride) || !ok8(a.o_batch_stride))
     return fail(FA_ERR_UNSUPPORTED, "q, o and the new k, v must start at 16-byte boundaries, with strides that are multiples of 8");
+
+  if (a.k_new)
+    if (int rc = check_written(c, a.k, a.v, outer, rows, a.h_k); rc != FA_OK) return rc;
 
   Kv8Params& p = out->p;
   p.a = a;
@@ -249,6 +264,7 @@ static int run_kv8_append(const fa_kv8_append_params& p_in, cudaStream_t st) {
     return fail(FA_ERR_UNSUPPORTED, "the codes of an 8-bit KV cache must start at 16-byte boundaries, with strides that are multiples of 16");
   if (p.total > 0x7fffffffLL || p.h_k > 32767) return fail(FA_ERR_UNSUPPORTED, "too many new tokens or heads in one call");
   if ((int64_t)p.kv_outer * p.rows > 0x7fffffffLL) return fail(FA_ERR_UNSUPPORTED, "too many tokens in the KV cache");
+  if (int rc = check_written(p.c, p.k_cache, p.v_cache, p.kv_outer, p.rows, p.h_k); rc != FA_OK) return rc;
   const int num_sm = p.num_sm > 0 ? p.num_sm : sm_count();
   int32_t* status = device_status_word();
   if (!status || num_sm <= 0) return fail(FA_ERR_CUDA, "cannot query the current device");

@@ -272,7 +272,8 @@ def quantized_kvcache_append(k, v, k_cache, v_cache, k_descale, v_descale, slot_
 
     slot_mapping (total,) int64: page * tokens of a page + row of each token, negative for rows of padding (skipped).  The new
     tokens of one block must be neighbours in the batch with consecutive slots, as ``paged_kvcache_plan`` gives them, and a
-    page that is written to must belong to one sequence.
+    page that is written to must belong to one sequence.  Expanded scales, or one tensor for K and V, are refused here (and with k, v in
+    ``flash_attn_with_kvcache``): they can only be read.
 
     A scale is the smallest power of two, 2^-40 at least, that brings the block's largest finite element into the codes' range
     (448 for e4m3, 127 for int8).  Where tokens are there in front of the new ones, the block keeps its scale if that is larger, and

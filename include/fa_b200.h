@@ -309,7 +309,8 @@ int fa_b200_kv8_fwd_alloc(const fa_fwd_params* p, const fa_kv8_cache* c, void* (
  * smallest power of two, 2^-40 at least, that brings the largest finite element into the codes' range (e4m3: 448, int8: 127).
  * A block whose first rows are not among the new ones keeps its scale if that is larger, else its earlier rows are
  * expressed in the new one; a block whose first row is written starts afresh.  Rows behind the new ones are not touched.  Codes are rounded to
- * nearest even; infinities saturate; NaN is stored as NaN (e4m3) or 0 (int8). */
+ * nearest even; infinities saturate; NaN is stored as NaN (e4m3) or 0 (int8).  K, V and the scales of every block and head need memory of their
+ * own: strides of 0 are for scales that are only read. */
 typedef struct fa_kv8_append_params {
   const void* k; /* (total, h_k, d), fp16 or bf16 */
   const void* v;

@@ -39,6 +39,17 @@ def _append(**change):
     return p
 
 
+OVERLAPS = [dict(ks_outer_stride=0), dict(vs_outer_stride=0), dict(ks_block_stride=0), dict(vs_block_stride=0), dict(ks_head_stride=0),
+            dict(vs_head_stride=0), dict(ks_outer_stride=0, ks_block_stride=0, ks_head_stride=0)]
+
+
+@pytest.mark.parametrize("change", OVERLAPS + [dict(v_cache=1 << 20), dict(v_scale=3 << 20)])
+def test_append_refuses_what_shares_memory(change):
+    """Scales of several blocks or heads, or of K and of V, in one place: many would read and write it at once."""
+    p = _append(**change)
+    assert "of its own" in _message(L.load().fa_b200_kv8_append(C.byref(p), None))
+
+
 @pytest.mark.parametrize("change", [dict(kc_outer_stride=0), dict(kc_row_stride=0), dict(vc_head_stride=0), dict(vc_row_stride=1032),
                                     dict(kc_head_stride=136), dict(kc_outer_stride=128 * 1024 + 8)])
 def test_append_takes_the_strides_that_its_header_says(change):
@@ -57,6 +68,26 @@ def _no_device(rc):
     dict(scale_block=128, ks_block_stride=0, vs_block_stride=0)])
 def test_append_strides_of_one_element_may_be_anything(change):
     assert _no_device(L.load().fa_b200_kv8_append(C.byref(_append(**change)), None))
+
+
+def _fwd_new(**change):
+    return _fwd(**{**dict(k=1 << 30, v=2 << 30, k_scale=3 << 20, v_scale=4 << 20, k_new=256, v_new=256, seqlen_new=1,
+                          knew_batch_stride=1024, knew_row_stride=1024, knew_head_stride=128, vnew_batch_stride=1024, vnew_row_stride=1024,
+                          vnew_head_stride=128, num_splits=1), **change})
+
+
+@pytest.mark.parametrize("change", OVERLAPS + [dict(v=1 << 30), dict(v_scale=3 << 20)])
+def test_new_tokens_refuse_what_shares_memory(change):
+    p, c = _fwd_new(**change)
+    assert "of its own" in _message(L.load().fa_b200_kv8_fwd(C.byref(p), C.byref(c), None, 0, None))
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="would launch")
+@pytest.mark.parametrize("change", OVERLAPS + [dict(v=256, k=256), dict(v_scale=256, k_scale=256)])
+def test_expanded_scales_may_be_read(change):
+    """A call without new tokens takes one scale for all blocks and heads, and one cache for K and V."""
+    p, c = _fwd(num_splits=1, **change)
+    assert _no_device(L.load().fa_b200_kv8_fwd(C.byref(p), C.byref(c), None, 0, None))
 
 
 RANDOM = r"""

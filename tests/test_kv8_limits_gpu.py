@@ -110,6 +110,35 @@ def test_new_tokens_on_pages_that_are_not_there(bad, s_q):
         U.check_attention(out[r], lse[r], U.attend(q[r], kv, kv, scale, True), tag=f"sequence {r}")
 
 
+@pytest.mark.parametrize("s_q", [1, 40])
+def test_expanded_scales_are_read_and_never_written(s_q):
+    """One scale for a whole cache, expanded to its blocks and heads, serves attention; calls that append refuse it and leave all as it was."""
+    g = _gen(52)
+    kc, _ = _random_cache(g, 5, 32, 2, 64, 2, INT8)
+    table, lens = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32), [60, 33]
+    one = torch.full((1,), 0.015625, device="cuda")
+    ks = one.expand(5, 2, 2)
+    kd, vd = kc.cuda(), kc.cuda()
+    q = torch.randn((2, s_q, 4, 64), generator=g).to(BF)
+    kw = dict(cache_seqlens=_i32(lens), page_table=table.cuda(), k_descale=ks, v_descale=ks, causal=True, return_softmax_lse=True)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kd, kd, **kw)
+    for r, n in enumerate(lens):
+        kv = _values(table[r], 32, n, kc, ks.cpu())
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv, kv, 0.125, True), tag=f"sequence {r}")
+    x, slots = torch.randn((2, 1, 2, 64), generator=g).to(BF).cuda(), torch.tensor([60, 97], device="cuda")
+    own = [torch.full((5, 2, 2), 0.015625, device="cuda") for _ in range(2)]
+    for c, s in (((kd, vd), (ks, own[1])), ((kd, vd), (own[0], ks)), ((kd, vd), (own[0], own[0])), ((kd, kd), own),
+                 ((kd, vd), (own[0][:1].expand(5, 2, 2), own[1])), ((kd, vd), (own[0][:, :1].expand(5, 2, 2), own[1]))):
+        with pytest.raises(RuntimeError, match="of its own"):
+            fa3.quantized_kvcache_append(x[:, 0], x[:, 0], *c, *s, slots)
+        with pytest.raises(RuntimeError, match="of its own"):
+            fa3.flash_attn_with_kvcache(q.cuda(), *c, x, x, **{**kw, "k_descale": s[0], "v_descale": s[1]})
+    for t in (kd, vd):
+        assert torch.equal(t.cpu(), kc)
+    assert all(bool((t == 0.015625).all()) for t in own + [one])
+    _status()
+
+
 # ---------------------------------------------------------------- attention
 @pytest.mark.parametrize("s_q", [1, 12, 40, 200])
 @pytest.mark.parametrize("bad", [9, -1])

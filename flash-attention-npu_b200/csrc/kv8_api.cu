@@ -85,6 +85,10 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
       return fail(FA_ERR_INVALID, "rotary_dim must be divisible by 16 and at most the head dimension");
     if (a.rotary_seqlen < a.seqlen_k) return fail(FA_ERR_INVALID, "rotary_cos / rotary_sin must have a row for every position of the cache");
   }
+  // Rows of a tile and keys of a block are counted in 32 bits.
+  const int64_t all_rows = (int64_t)std::max(a.seqlen_q, a.cu_seqlens_q ? a.total_q : 0) * (a.h / a.h_k);
+  if (all_rows > 0x3fffffff) return fail(FA_ERR_UNSUPPORTED, "too many query rows in one call");
+  if (a.seqlen_k > 0x7fffffff - 4096) return fail(FA_ERR_UNSUPPORTED, "too many tokens in a sequence's part of the KV cache");
   const int rows = a.block_table ? a.page_size : a.seqlen_k;
   const int64_t outer = a.kv_outer > 0 ? a.kv_outer : a.b;
   if (int rc = check_cache(c, rows, a.d); rc != FA_OK) return rc;

@@ -127,6 +127,7 @@ bool fill_params(const FwdArgs& a, fa_fwd_params& p) {
   p.dtype = q.scalar_type() == at::kBFloat16 ? FA_BF16 : FA_FP16;
   if (packed_q) {
     p.q_row_stride = q.stride(0); p.q_head_stride = q.stride(1);
+    if (a.kv8 && a.max_q > INT32_MAX) return false;
     p.seqlen_q = (int32_t)a.max_q; p.total_q = (int32_t)q.size(0);
   } else {
     p.q_batch_stride = q.stride(0); p.q_row_stride = q.stride(1); p.q_head_stride = q.stride(2);
@@ -142,6 +143,7 @@ bool fill_params(const FwdArgs& a, fa_fwd_params& p) {
     if (a.table || a.batch_idx) p.kv_outer = (int32_t)k.size(0);
     p.seqlen_k = (int32_t)k.size(1);
     if (a.table) {
+      if (a.kv8 && a.table->size(1) * k.size(1) > INT32_MAX) return false;
       p.page_size = (int32_t)k.size(1);
       p.seqlen_k = (int32_t)(a.table->size(1) * k.size(1));
       p.block_table_batch_stride = a.table->stride(0);
@@ -498,7 +500,7 @@ PyObject* step_plan(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (n != 7 || !plain_eager()) return not_implemented();
   if (!as_tensor(o[0], have) || !as_tensor(o[1], add) || !as_tensor(o[2], table) || !as_tensor(o[3], free) || !as_int(o[4], page) ||
       !as_int(o[5], total) || !as_tensor(o[6], num_free) || !have || !add || !table || !free || !plain(*table) ||
-      table->scalar_type() != at::kInt || table->dim() != 2 || total < 0 || page <= 0 || page > INT32_MAX)
+      table->scalar_type() != at::kInt || table->dim() != 2 || total < 0 || total > INT32_MAX || page <= 0 || page > INT32_MAX)
     return not_implemented();
   const int64_t b = have->numel(), cols = table->size(1);
   if (!index_tensor(have, *table, b) || !index_tensor(add, *table, b) || !index_tensor(free, *table, free->numel()) ||

@@ -13,6 +13,7 @@ import torch
 from . import lib as L
 from . import ops
 
+INT32_MAX = 2 ** 31 - 1
 CODES = {torch.float8_e4m3fn: L.CODE_E4M3, torch.int8: L.CODE_INT8}
 
 
@@ -85,6 +86,10 @@ def attention_forward_kv8(q, k_cache, v_cache, k_descale, v_descale, *, k_new=No
             raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape (batch_size,)")
     if block_table is not None and (block_table.dim() != 2 or block_table.shape[0] != b):
         raise RuntimeError("page_table must have shape (batch_size, max_num_pages_per_seq)")
+    if cu_seqlens_q is not None and max_seqlen_q is not None and int(max_seqlen_q) > INT32_MAX:
+        raise RuntimeError("too many query rows in one call")
+    if block_table is not None and block_table.shape[1] * k_cache.shape[1] > INT32_MAX:
+        raise RuntimeError("too many tokens in a sequence's part of the KV cache")
     if block_table is None and cache_batch_idx is None and k_cache.shape[0] != b:
         raise RuntimeError("a contiguous KV cache needs one row per sequence, or cache_batch_idx")
     if (k_new is None) != (v_new is None):
@@ -157,9 +162,11 @@ def kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, 
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b or page_table.stride(1) != 1 or (
             b > 1 and page_table.stride(0) < page_table.shape[1]):
         raise RuntimeError("page_table must be an int32 tensor of shape (batch_size, max_num_pages_per_seq) whose rows do not overlap")
-    total = int(total_new)
+    total, page_size = int(total_new), int(page_size)
     if total < 0:
         raise RuntimeError("total_new must not be negative")
+    if not 0 < page_size <= INT32_MAX or total > INT32_MAX:
+        raise RuntimeError("bad sizes of the page table, the free list or the packed batch")
     i32 = dict(dtype=torch.int32, device=dev)
     slots, positions = torch.empty(total, dtype=torch.int64, device=dev), torch.empty(total, **i32)
     cu, after, taken = torch.empty(b + 1, **i32), torch.empty(b, **i32), torch.empty(1, **i32)
@@ -168,7 +175,7 @@ def kvcache_plan(cache_seqlens, new_seqlens, page_table, free_pages, page_size, 
     p.num_free = ops._ptr(num_free)
     p.slots, p.cu_new, p.after, p.positions, p.pages_taken = (t.data_ptr() for t in (slots, cu, after, positions, taken))
     p.table_stride, p.total = page_table.stride(0), total
-    p.b, p.cols, p.page_size, p.n_free = b, page_table.shape[1], int(page_size), free_pages.numel()
+    p.b, p.cols, p.page_size, p.n_free = b, page_table.shape[1], page_size, free_pages.numel()
     p.num_sm = ops._num_sm(dev)
     with torch.cuda.device(dev):
         L.check(lib.fa_b200_kvcache_plan(C.byref(p), torch.cuda.current_stream(dev).cuda_stream))

@@ -90,6 +90,15 @@ def test_expanded_scales_may_be_read(change):
     assert _no_device(L.load().fa_b200_kv8_fwd(C.byref(p), C.byref(c), None, 0, None))
 
 
+@pytest.mark.parametrize("change,said", [
+    (dict(seqlen_q=1 << 30, lse_batch_stride=32 << 30, lse_head_stride=1 << 30), "too many query rows"),
+    (dict(cu_seqlens_q=256, total_q=1 << 29, lse_head_stride=1 << 29), "too many query rows"),
+    (dict(seqlen_k=(1 << 31) - 128, k_batch_stride=1 << 41, v_batch_stride=1 << 41, b=1, h=1, h_k=1, total_q=1), "too many tokens")])
+def test_sizes_beyond_the_index_arithmetic_are_refused(change, said):
+    p, c = _fwd(**change)
+    assert said in _message(L.load().fa_b200_kv8_fwd(C.byref(p), C.byref(c), None, 0, None))
+
+
 RANDOM = r"""
 #include <cstdio>
 #include <initializer_list>

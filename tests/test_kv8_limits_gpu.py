@@ -71,6 +71,27 @@ def test_plan_of_negative_lengths(have, new):
     assert cu.tolist() == [0, at, at + 2] and slots.tolist() == ([-1] * at + [36, 37] + [-1] * 6)[:6]
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    table, lens = torch.zeros((2, 4), dtype=torch.int32, device="cuda"), _i32([1, 1])
+    for page in (2 ** 32 + 16, -2 ** 32 + 16):
+        with pytest.raises(RuntimeError, match="sizes"):
+            fa3.paged_kvcache_plan(lens, lens, table, lens, page, 4)
+    with pytest.raises(RuntimeError, match="sizes"):
+        fa3.paged_kvcache_plan(lens, lens, table, lens, 16, 2 ** 31)
+    codes, scales = torch.zeros((4, 16, 1, 16), dtype=torch.int8, device="cuda"), torch.ones((4, 1, 1), device="cuda")
+    for most in (2 ** 32 + 1, -1, 2 ** 30):
+        with pytest.raises(RuntimeError, match="sequence length|query rows"):
+            fa3.flash_attn_with_kvcache(torch.zeros((40, 2, 16), dtype=BF, device="cuda"), codes, codes, cache_seqlens=lens, page_table=table,
+                                        cu_seqlens_q=_i32([0, 20, 40]), max_seqlen_q=most, k_descale=scales, v_descale=scales)
+    # a page table whose columns cover 2^32 + 2^14 tokens
+    kc = torch.zeros((2, 1 << 14, 1, 16), dtype=torch.int8, device="cuda")
+    ks = torch.ones((2, 1, 1), device="cuda")
+    table = torch.zeros((1, (1 << 18) + 1), dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="too many tokens"):
+        fa3.flash_attn_with_kvcache(torch.zeros((1, 1, 1, 16), dtype=BF, device="cuda"), kc, kc, cache_seqlens=_i32([40]), page_table=table,
+                                    k_descale=ks, v_descale=ks)
+
+
 # ---------------------------------------------------------------- append
 def test_append_to_slots_that_are_not_there():
     """Slots at and behind the cache's end are skipped and reported; what is around stays as it was."""

@@ -30,7 +30,8 @@ def fwd(q, k, v, k_new_, v_new_, q_v_, out_, cu_seqlens_q_, cu_seqlens_k_, cu_se
 
     q is (b, s_q, h, d), or (total_q, h, d) with cu_seqlens_q_; k / v are dense, varlen
     (with cu_seqlens_k_), a contiguous cache or a paged cache (with page_table_); seqused_k_ gives
-    the per-sequence key counts.  softmax_lse is (b, h, s_q) or (h, total_q).
+    the per-sequence key counts.  softmax_lse is (b, h, s_q) or (h, total_q).  A contiguous or paged cache may hold 8-bit codes, with
+    k_descale_ / v_descale_ as their scales: flash_attn_with_kvcache comes here so.
     """
     # same rejections as the reference (:150-162)
     _reject(q_v_ is not None, "NPU FlashAttention does not support qv")

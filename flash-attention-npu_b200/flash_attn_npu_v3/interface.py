@@ -35,6 +35,9 @@ def _forward(q, k, v, k_new=None, v_new=None, qv=None, out_=None, cu_seqlens_q=N
              seqlens_rotary=None, q_descale=None, k_descale=None, v_descale=None, softmax_scale=None, causal=False,
              window_size_left=-1, window_size_right=-1, attention_chunk=0, softcap=0.0, rotary_interleaved=True,
              scheduler_metadata=None, num_splits=1, pack_gqa=None, sm_margin=0):
+    if kv8.holds_codes(k, v):  # (flash_attn_with_kvcache does not come here with an 8-bit cache)
+        _ext._reject(q_descale is not None or k_descale is not None or v_descale is not None, "NPU FlashAttention does not support descale")
+        raise RuntimeError("query and key/value must have the same dtype")
     q, k, v, k_new, v_new = [maybe_contiguous(x) for x in (q, k, v, k_new, v_new)]
     cu_seqlens_q, cu_seqlens_k, seqused_k, page_table, kv_batch_idx = [
         maybe_contiguous(x) for x in (cu_seqlens_q, cu_seqlens_k, seqused_k, page_table, kv_batch_idx)]

@@ -99,6 +99,15 @@ def test_sizes_beyond_the_index_arithmetic_are_refused(change, said):
     assert said in _message(L.load().fa_b200_kv8_fwd(C.byref(p), C.byref(c), None, 0, None))
 
 
+def test_differentiable_calls_refuse_codes():
+    q, kc, s = torch.zeros(2, 32, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 32, 2, 64, dtype=torch.int8), torch.ones(2, 1, 2)
+    with pytest.raises(RuntimeError, match="does not support descale"):
+        fa3.flash_attn_func(q, kc, kc, k_descale=s, v_descale=s)
+    cu = torch.tensor([0, 32, 64], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="does not support descale"):
+        fa3.flash_attn_varlen_func(q.flatten(0, 1), kc.flatten(0, 1), kc.flatten(0, 1), cu, cu, 32, 32, k_descale=s, v_descale=s)
+
+
 RANDOM = r"""
 #include <cstdio>
 #include <initializer_list>

@@ -246,3 +246,18 @@ def test_windows_about_the_longest_sequence(s_q, h, left, right):
     for r in range(3):
         U.check_attention(out[r], lse[r], U.attend(q[r], kv[r], kv[r], 0.125, is_causal, (wl, wr) if is_local else None), tag=f"sequence {r}")
     _status()
+
+
+# ---------------------------------------------------------------- other calls
+def test_codes_are_for_kv_cache_calls_only():
+    """The differentiable calls refuse codes with and without scales, also where a gradient is wanted."""
+    kc, s = torch.zeros((2, 32, 2, 64), dtype=INT8, device="cuda"), torch.ones((2, 1, 2), device="cuda")
+    cu = _i32([0, 32, 64])
+    for grad in (False, True):
+        q = torch.zeros((2, 32, 4, 64), dtype=BF, device="cuda", requires_grad=grad)
+        with pytest.raises(RuntimeError, match="does not support descale"):
+            fa3.flash_attn_func(q, kc, kc, k_descale=s, v_descale=s)
+        with pytest.raises(RuntimeError, match="same dtype"):
+            fa3.flash_attn_func(q, kc, kc)
+        with pytest.raises(RuntimeError, match="does not support descale"):
+            fa3.flash_attn_varlen_func(q.flatten(0, 1), kc.flatten(0, 1), kc.flatten(0, 1), cu, cu, 32, 32, k_descale=s, v_descale=s)

@@ -184,10 +184,21 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
     reach others whose mask hides it (their weight is 0, and 0 * NaN is NaN).  scheduler_metadata and q_descale are refused."""
     if softmax_scale is None:
         softmax_scale = _default_scale(q, qv)
-    if kv8.holds_codes(k_cache, v_cache):
-        if (qv is None and cache_leftpad is None and cu_seqlens_k_new is None and rotary_seqlens is None and q_descale is None
-                and attention_chunk == 0 and scheduler_metadata is None and not isinstance(cache_seqlens, int)
-                and not torch.compiler.is_compiling()):
+    eager = (qv is None and cache_leftpad is None and cu_seqlens_k_new is None and rotary_seqlens is None and q_descale is None
+             and attention_chunk == 0 and not isinstance(cache_seqlens, int) and not torch.compiler.is_compiling())
+    if (eager and k_descale is None and v_descale is None
+            # (the bytes of a plan can only be read from a plain tensor outside every mode)
+            and (scheduler_metadata is None or (type(scheduler_metadata) is torch.Tensor and _native.plain_eager()))):
+        plan = None if scheduler_metadata is None else _ext._plan_bytes(scheduler_metadata)
+        r = _native.kvcache(q, k_cache, v_cache, k, v, cu_seqlens_q, max_seqlen_q, cache_seqlens, cache_batch_idx, page_table,
+                            rotary_cos, rotary_sin, rotary_interleaved, None, softmax_scale, causal, window_size[0],
+                            window_size[1], softcap, num_splits, plan, True)
+        if r is not NotImplemented:
+            if not return_softmax_lse:
+                return r[0]
+            return (*r, torch.empty((0,), device=q.device), torch.empty((0,), device=q.device))
+    if kv8.holds_codes(k_cache, v_cache):  # (behind the 16-bit calls, which it would cost half a microsecond; the native path declines codes)
+        if eager and scheduler_metadata is None:
             r = _native.kvcache8(q, k_cache, v_cache, k, v, cu_seqlens_q, max_seqlen_q, cache_seqlens, cache_batch_idx, page_table,
                                  rotary_cos, rotary_sin, rotary_interleaved, k_descale, v_descale, softmax_scale, causal,
                                  window_size[0], window_size[1], softcap, num_splits, return_softmax_lse)
@@ -200,19 +211,6 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
         if not return_softmax_lse:
             return out
         return out, lse, torch.empty((0,), device=q.device), torch.empty((0,), device=q.device)
-    if (qv is None and cache_leftpad is None and cu_seqlens_k_new is None and rotary_seqlens is None and q_descale is None
-            and k_descale is None and v_descale is None and attention_chunk == 0 and not isinstance(cache_seqlens, int)
-            and not torch.compiler.is_compiling()
-            # (the bytes of a plan can only be read from a plain tensor outside every mode)
-            and (scheduler_metadata is None or (type(scheduler_metadata) is torch.Tensor and _native.plain_eager()))):
-        plan = None if scheduler_metadata is None else _ext._plan_bytes(scheduler_metadata)
-        r = _native.kvcache(q, k_cache, v_cache, k, v, cu_seqlens_q, max_seqlen_q, cache_seqlens, cache_batch_idx, page_table,
-                            rotary_cos, rotary_sin, rotary_interleaved, None, softmax_scale, causal, window_size[0],
-                            window_size[1], softcap, num_splits, plan, True)
-        if r is not NotImplemented:
-            if not return_softmax_lse:
-                return r[0]
-            return (*r, torch.empty((0,), device=q.device), torch.empty((0,), device=q.device))
     assert k_cache.stride(-1) == 1, "k_cache must have contiguous last dimension"
     assert v_cache.stride(-1) == 1, "v_cache must have contiguous last dimension"
     if cache_seqlens is not None and isinstance(cache_seqlens, int):

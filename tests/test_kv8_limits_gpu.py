@@ -261,3 +261,12 @@ def test_codes_are_for_kv_cache_calls_only():
             fa3.flash_attn_func(q, kc, kc)
         with pytest.raises(RuntimeError, match="does not support descale"):
             fa3.flash_attn_varlen_func(q.flatten(0, 1), kc.flatten(0, 1), kc.flatten(0, 1), cu, cu, 32, 32, k_descale=s, v_descale=s)
+
+
+def test_a_16_bit_call_asks_nothing_of_an_8_bit_one(monkeypatch):
+    """The native path is tried before anything is asked about codes."""
+    x = torch.randn((2, 64, 2, 64), generator=_gen(49)).to(BF).cuda()
+    q = torch.randn((2, 1, 4, 64), generator=_gen(50)).to(BF).cuda()
+    want = fa3.flash_attn_with_kvcache(q, x, x, cache_seqlens=_i32([60, 33]))
+    monkeypatch.setattr(kv8, "holds_codes", None)
+    assert torch.equal(fa3.flash_attn_with_kvcache(q, x, x, cache_seqlens=_i32([60, 33])), want)

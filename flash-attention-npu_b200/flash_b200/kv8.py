@@ -54,10 +54,10 @@ def _cache_block(k_cache, v_cache, k_descale, v_descale, like: Optional[torch.Te
 
 
 def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """The kernels read 16 bytes at a time."""
-    if t is None or (t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
+    """The kernels read 16 bytes at a time; strides count for dimensions of one element too."""
+    if t is None or (t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1])):
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
 def attention_forward_kv8(q, k_cache, v_cache, k_descale, v_descale, *, k_new=None, v_new=None, cu_seqlens_q=None, max_seqlen_q=None,

@@ -108,6 +108,16 @@ def test_differentiable_calls_refuse_codes():
         fa3.flash_attn_varlen_func(q.flatten(0, 1), kc.flatten(0, 1), kc.flatten(0, 1), cu, cu, 32, 32, k_descale=s, v_descale=s)
 
 
+def test_odd_strides_of_dimensions_of_one_element_are_put_right():
+    base = torch.arange(4096, dtype=torch.float32).to(torch.bfloat16)
+    for shape, strides in (((1, 1, 4, 64), (1001, 333, 64, 1)), ((2, 1, 1, 64), (128, 7, 3, 1)), ((1, 4, 64), (5, 64, 1))):
+        t = torch.as_strided(base, shape, strides)
+        a = kv8._aligned(t)
+        assert torch.equal(a, t) and all(s % 8 == 0 for s in a.stride()[:-1]) and a.data_ptr() % 16 == 0
+    t = base[:512].view(2, 4, 64)
+    assert kv8._aligned(t) is t
+
+
 RANDOM = r"""
 #include <cstdio>
 #include <initializer_list>

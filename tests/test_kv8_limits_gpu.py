@@ -248,6 +248,24 @@ def test_windows_about_the_longest_sequence(s_q, h, left, right):
     _status()
 
 
+def test_odd_strides_of_dimensions_of_one_element():
+    """... are put right on the way, as rows of a wider tensor are."""
+    g = _gen(53)
+    kc, ks, _, kv = _cache_for(g, [100], 0, 32, 2, 64, E4M3)
+    big = torch.randn(3000, generator=g).to(BF)
+    q, kn = torch.as_strided(big, (1, 1, 8, 64), (1001, 333, 64, 1)), torch.as_strided(big, (1, 1, 2, 64), (77, 5, 72, 1), 1024)
+    dev = big.cuda()
+    qd, knd = torch.as_strided(dev, (1, 1, 8, 64), (1001, 333, 64, 1)), torch.as_strided(dev, (1, 1, 2, 64), (77, 5, 72, 1), 1024)
+    got = [kc.cuda(), kc.cuda(), ks.cuda(), ks.cuda()]
+    out, lse, *_ = fa3.flash_attn_with_kvcache(qd, *got[:2], knd, knd, cache_seqlens=_i32([64]), k_descale=got[2], v_descale=got[3], causal=True,
+                                               return_softmax_lse=True)
+    U.append(kn[0], kc, ks, [64])
+    x = torch.stack([U.values_of(kc[0, t]) * ks[0, t // 32].double()[:, None] for t in range(65)])
+    U.check_attention(out[0], lse[0], U.attend(q[0], x, x, 0.125, True))
+    for c, s in (got[0::2], got[1::2]):
+        assert torch.equal(s.cpu()[0, :3], ks[0, :3]) and torch.equal(U.values_of(c.cpu()[0, :65]), U.values_of(kc[0, :65]))
+
+
 # ---------------------------------------------------------------- other calls
 def test_codes_are_for_kv_cache_calls_only():
     """The differentiable calls refuse codes with and without scales, also where a gradient is wanted."""

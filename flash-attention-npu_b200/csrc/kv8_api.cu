@@ -122,8 +122,8 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   }
   bool is_causal = false, is_local = false;
   window_rule(a.seqlen_q, max_k, a.causal != 0, wl, wr, is_causal, is_local);
-  p.wl = wl;
-  p.wr = wr;
+  p.wl = std::max(wl, -(1 << 30));  // (sums with positions stay within 32 bits)
+  p.wr = std::max(wr, -(1 << 30));
 
   // ---- tile and key splits ----
   const int rows_max = a.seqlen_q * p.group;

@@ -104,6 +104,8 @@ bool fill_params(const FwdArgs& a, fa_fwd_params& p) {
   const bool packed_q = a.cu_q != nullptr, packed_k = a.cu_k != nullptr;
   if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16) return false;
   if (q.dim() != (packed_q ? 3 : 4)) return false;
+  auto in_32_bits = [](int64_t x) { return x == (int32_t)x; };
+  if (a.kv8 && !(in_32_bits(a.max_q) && in_32_bits(a.wl) && in_32_bits(a.wr) && in_32_bits(a.num_splits))) return false;
   if (a.kv8 ? !code_tensor(a.k, q) || !code_tensor(a.v, q) || a.k->scalar_type() != a.v->scalar_type()
             : !data_tensor(a.k, q, packed_k ? 3 : 4) || !data_tensor(a.v, q, packed_k ? 3 : 4))
     return false;
@@ -127,7 +129,6 @@ bool fill_params(const FwdArgs& a, fa_fwd_params& p) {
   p.dtype = q.scalar_type() == at::kBFloat16 ? FA_BF16 : FA_FP16;
   if (packed_q) {
     p.q_row_stride = q.stride(0); p.q_head_stride = q.stride(1);
-    if (a.kv8 && a.max_q > INT32_MAX) return false;
     p.seqlen_q = (int32_t)a.max_q; p.total_q = (int32_t)q.size(0);
   } else {
     p.q_batch_stride = q.stride(0); p.q_row_stride = q.stride(1); p.q_head_stride = q.stride(2);

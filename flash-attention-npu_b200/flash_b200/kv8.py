@@ -103,6 +103,8 @@ def attention_forward_kv8(q, k_cache, v_cache, k_descale, v_descale, *, k_new=No
             raise RuntimeError(f"{name} must be a contiguous 2-D tensor with the dtype and device of q")
     if rotary_cos is not None and rotary_sin is not None and rotary_cos.shape != rotary_sin.shape:
         raise RuntimeError("rotary_cos and rotary_sin must have the same shape")
+    # Python's numbers, in the 32 bits that they go into: a window beyond is as wide as one can be
+    window_left, window_right, num_splits = (max(-INT32_MAX, min(INT32_MAX, int(x))) for x in (window_left, window_right, num_splits))
     q, k_new, v_new = _aligned(q), _aligned(k_new), _aligned(v_new)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(ops._lse_shape(q, cu_seqlens_q is not None), dtype=torch.float32, device=q.device)

@@ -248,6 +248,21 @@ def test_windows_about_the_longest_sequence(s_q, h, left, right):
     _status()
 
 
+@pytest.mark.parametrize("s_q,h", [(8, 4), (40, 4)])
+@pytest.mark.parametrize("left,right,sees", [(2 ** 32, 0, "causal"), (2 ** 63 - 1, 0, "causal"), (2 ** 32 + 5, 2 ** 40, "all"), (-2 ** 32, -2 ** 40 - 1, "all"),
+                                             (-2 ** 31, 3, "nothing"), (-2 ** 32 + 4, 3, "nothing"), (4, -2 ** 31, "nothing"), (4, -2 ** 33 + 4, "nothing")])
+def test_windows_at_and_beyond_32_bits(left, right, sees, s_q, h):
+    """Numbers that 32 bits cannot hold mean what they say, and so do sums of positions with those that are just held."""
+    g = _gen(54)
+    kc, ks, table, kv = _cache_for(g, [100], 64, 32, 2, 64, E4M3)
+    table = torch.cat([table, torch.full((1, 14), 2 ** 30, dtype=torch.int32)], 1)
+    q = torch.randn((1, s_q, h, 64), generator=g).to(BF)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), kc.cuda(), cache_seqlens=_i32([100]), page_table=table.cuda(), k_descale=ks.cuda(),
+                                               v_descale=ks.cuda(), window_size=(left, right), return_softmax_lse=True)
+    U.check_attention(out[0], lse[0], U.attend(q[0], kv[0], kv[0], 0.125, sees == "causal", (-200, -200) if sees == "nothing" else None))
+    _status()
+
+
 def test_odd_strides_of_dimensions_of_one_element():
     """... are put right on the way, as rows of a wider tensor are."""
     g = _gen(53)

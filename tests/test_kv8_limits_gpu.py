@@ -229,6 +229,75 @@ def test_offsets_out_of_range(cu, most, rows, splits):
             U.check_attention(out[a:a + upto], lse[:, a:a + upto], (want[0][:upto], want[1][:, :upto], want[2][:upto]), tag=f"sequence {r}")
 
 
+@pytest.mark.parametrize("s_q", [1, 4, 8, 33])
+@pytest.mark.parametrize("form", ["none", "int"])
+def test_lengths_by_default_and_as_a_number(form, s_q):
+    g = _gen(45)
+    kc, ks, _, kv = _cache_for(g, [96, 96], 0, 16, 2, 64, E4M3)
+    q = torch.randn((2, s_q, 8, 64), generator=g).to(BF)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), kc.cuda(), cache_seqlens=None if form == "none" else 77, k_descale=ks.cuda(),
+                                               v_descale=ks.cuda(), causal=True, return_softmax_lse=True)
+    n = 96 if form == "none" else 77
+    for r in range(2):
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv[r][:n], kv[r][:n], 0.125, True), tag=f"sequence {r}")
+    _status()
+
+
+@pytest.mark.parametrize("s_q", [1, 5, 20, 40, 150])
+@pytest.mark.parametrize("up", [1.0, 2.0 ** 60, 2.0 ** -70, -1.0])
+def test_numbers_of_every_size(s_q, up):
+    """Queries whose elements span bf16's range, scales from 2^-40 to 2^30 within one sequence with zero scales and blocks of zeros among them, scores in
+    the hundreds, negative softmax scales, for every number of rows.
+
+    Allowed, beside the output's half step and P's rounding to fp16 (2^-11 of every p |v|):
+    scores: sums over four steps of 16 products, each step off by at most 2^-22 of the sum S of all |q k| (fp32, truncated), so by 2^-20 S, which a
+    weight is off by twice (itself and the sum) and the LSE once;
+    small P': P' has fp16's subnormals below, off by at most 2^-25 of a unit in which the largest P' is 2^7 at least, so by 2^-32 of the largest p * scale for
+    each code."""
+    g = _gen(int(s_q))
+    n, d = 512, 64
+    kc, ks, _, _ = _cache_for(g, [n], 0, 16, 1, d, E4M3)
+    vs = torch.exp2(torch.linspace(-40, 30, n // 16).round())[None, :, None]
+    vs[0, 5] = 0.0
+    vc = torch.randn((1, n, 1, d), generator=g).clamp(-3, 3).to(E4M3)
+    vc[0, 48:64] = 0.0
+    k64 = U.values_of(kc[0]) * ks[0].double().repeat_interleave(16, 0)[:, :, None]
+    each = vs[0].double().repeat_interleave(16, 0)  # (n, 1)
+    c64 = U.values_of(vc[0])
+    q = torch.randn((1, s_q, 8, d), generator=g)
+    q[..., :8] *= 2.0 ** -12
+    q = (q * abs(up)).to(BF)
+    scale = 1.5 / up
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), vc.cuda(), cache_seqlens=_i32([n]), k_descale=ks.cuda(), v_descale=vs.cuda(),
+                                               softmax_scale=scale, causal=True, return_softmax_lse=True)
+    o64, l64, size = U.attend(q[0], k64, c64 * each[:, :, None], scale, True)
+    seen = torch.arange(n)[None] <= torch.arange(s_q)[:, None] + n - s_q
+    q64, half = q[0].double(), torch.finfo(BF).eps / 2
+    for h in range(8):
+        x = torch.where(seen, q64[:, h] @ k64[:, 0].T * scale, -math.inf)
+        small = 2.0 ** -32 * (torch.softmax(x, -1) * each[:, 0]).amax(-1, keepdim=True) * c64[:, 0].abs().sum(0)
+        score = 2.0 ** -20 * (q64[:, h].abs() @ k64[:, 0].abs().T * abs(scale)).amax(-1, keepdim=True)
+        off = (out[0, :, h].double().cpu() - o64[:, h]).abs()
+        allowed = half * o64[:, h].abs() + ((2.0 ** -11 + 2 * score) * size[:, h] + small) * (1 + half) + 2.0 ** -24
+        assert bool((off <= allowed).all()), (h, float((off / allowed).max()))
+        off = (lse[0, h].double().cpu() - l64[h]).abs()
+        assert bool((off <= 2.0 ** -16 + 2.0 ** -22 * l64[h].abs() + score[:, 0]).all()), (h, float(off.max()))
+    _status()
+
+
+@pytest.mark.parametrize("s_q", [1, 4, 8, 33])
+@pytest.mark.parametrize("softcap", [0.0, 25.0])
+def test_negative_softmax_scale(s_q, softcap):
+    g = _gen(46)
+    kc, ks, table, kv = _cache_for(g, [300, 41], 32, 32, 2, 128, INT8, pow2=False)
+    q = torch.randn((2, s_q, 16, 128), generator=g).to(FP)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), kc.cuda(), kc.cuda(), cache_seqlens=_i32([300, 41]), page_table=table.cuda(), k_descale=ks.cuda(),
+                                               v_descale=ks.cuda(), softmax_scale=-0.1, softcap=softcap, causal=True, return_softmax_lse=True)
+    for r in range(2):
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv[r], kv[r], -0.1, True, softcap=softcap), softcap, f"sequence {r}")
+    _status()
+
+
 @pytest.mark.parametrize("s_q,h", [(1, 4), (7, 8), (20, 8), (150, 4)])
 @pytest.mark.parametrize("left,right", [(299, -1), (300, -1), (298, -1), (298, 0), (299, 0), (-5, 3), (-3, 3), (-40, 3), (2, -2)])
 def test_windows_about_the_longest_sequence(s_q, h, left, right):
@@ -261,6 +330,20 @@ def test_windows_at_and_beyond_32_bits(left, right, sees, s_q, h):
                                                v_descale=ks.cuda(), window_size=(left, right), return_softmax_lse=True)
     U.check_attention(out[0], lse[0], U.attend(q[0], kv[0], kv[0], 0.125, sees == "causal", (-200, -200) if sees == "nothing" else None))
     _status()
+
+
+@pytest.mark.parametrize("s_q,h,d", [(1, 8, 128), (4, 16, 128), (4, 16, 64), (16, 8, 64), (150, 8, 128), (40, 8, 256), (1, 8, 256)])
+def test_a_call_repeats_itself(s_q, h, d):
+    """Bit for bit, with another call of other inputs in between."""
+    g = _gen(48)
+    kc, ks, table, _ = _cache_for(g, [900, 77, 300], 32, 16, 2, d, E4M3)
+    kd, sd = kc.cuda(), ks.cuda()
+    qs = [torch.randn((3, s_q, h, d), generator=g).to(BF).cuda() for _ in range(2)]
+    call = lambda i: fa3.flash_attn_with_kvcache(qs[i], kd, kd, cache_seqlens=_i32([900, 77, 300]), page_table=table.cuda(), k_descale=sd,  # noqa: E731
+                                                 v_descale=sd, causal=True, return_softmax_lse=True)[:2]
+    first, _, again = call(0), call(1), call(0)
+    for a, b in zip(first, again):
+        assert torch.equal(_raw(a), _raw(b))
 
 
 def test_odd_strides_of_dimensions_of_one_element():

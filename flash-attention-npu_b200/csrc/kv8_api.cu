@@ -72,6 +72,8 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   if (a.cache_batch_idx && (a.block_table || a.kv_outer <= 0))
     return fail(FA_ERR_INVALID, "cache_batch_idx needs a contiguous cache and kv_outer = the number of cache rows");
   if (a.kv_outer < 0) return fail(FA_ERR_INVALID, "negative kv_outer");
+  if (!a.block_table && !a.cache_batch_idx && a.kv_outer > 0 && a.kv_outer < a.b)
+    return fail(FA_ERR_INVALID, "a contiguous KV cache needs one row per sequence, or cache_batch_idx");
   if ((a.k_new != nullptr) != (a.v_new != nullptr)) return fail(FA_ERR_INVALID, "k and v must be passed together");
   if (a.k_new && a.seqlen_new <= 0) return fail(FA_ERR_INVALID, "seqlen_new must be positive when k, v are given");
   if (!a.k_new && a.seqlen_new != 0) return fail(FA_ERR_INVALID, "seqlen_new given without k, v");
@@ -288,6 +290,7 @@ static int run_kvcache_plan(const fa_kvcache_plan_params& p, cudaStream_t st) {
   if (!p.have || !p.add || (!p.table && p.cols) || (!p.free_pages && p.n_free) || ((!p.slots || !p.positions) && p.total) || !p.cu_new || !p.after ||
       !p.pages_taken)
     return fail(FA_ERR_INVALID, "an input or output of the plan is null");
+  if (p.b > 1 && p.table_stride < p.cols) return fail(FA_ERR_INVALID, "the rows of the page table must not overlap");
   const int num_sm = p.num_sm > 0 ? p.num_sm : sm_count();
   int32_t* status = device_status_word();
   if (!status || num_sm <= 0) return fail(FA_ERR_CUDA, "cannot query the current device");

@@ -99,6 +99,21 @@ def test_sizes_beyond_the_index_arithmetic_are_refused(change, said):
     assert said in _message(L.load().fa_b200_kv8_fwd(C.byref(p), C.byref(c), None, 0, None))
 
 
+def test_caches_and_tables_that_are_too_small_are_refused():
+    """A contiguous cache of fewer rows than sequences, a page table whose rows run into one another."""
+    lib = L.load()
+    for new in ({}, dict(k_new=256, v_new=256, seqlen_new=1)):
+        p, c = _fwd(kv_outer=1, **new)
+        assert "one row per sequence" in _message(lib.fa_b200_kv8_fwd(C.byref(p), C.byref(c), None, 0, None))
+    p = L.KvcachePlanParams()
+    for n in ("have", "add", "table", "free_pages", "slots", "cu_new", "after", "positions", "pages_taken"):
+        setattr(p, n, 256)
+    p.total, p.b, p.cols, p.page_size, p.n_free, p.num_sm = 4, 4, 16, 16, 8, 148
+    for stride in (0, 15, -16):
+        p.table_stride = stride
+        assert "overlap" in _message(lib.fa_b200_kvcache_plan(C.byref(p), None))
+
+
 def test_differentiable_calls_refuse_codes():
     q, kc, s = torch.zeros(2, 32, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 32, 2, 64, dtype=torch.int8), torch.ones(2, 1, 2)
     with pytest.raises(RuntimeError, match="does not support descale"):

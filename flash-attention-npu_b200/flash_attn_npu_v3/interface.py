@@ -177,7 +177,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
     (the last two are empty tensors, as in the reference :1095).
 
     k_cache / v_cache may hold 8-bit codes (torch.float8_e4m3fn or torch.int8) with k_descale / v_descale fp32 of shape
-    (pages or cache rows, blocks of tokens, nheads_k): an element stands for code * scale of its (block, head).  Blocks have
+    (pages or cache rows, blocks of tokens, nheads_k): an element stands for code * scale of its (block, head).  Scales are
+    positive or zero, never negative, and V's below 2^-64 count as 2^-64; they may be expanded tensors where nothing is appended.  Blocks have
     equal, whole multiples of 16 tokens: a page (or a cache row) divided by the second dimension.  Head dims are multiples of 16.  k / v are then
     appended as ``quantized_kvcache_append`` does -- codes and scales change in place -- and attended to as the cache
     holds them.  Codes of tokens that no query of the sequence sees may be anything; a NaN code of a value that some query sees may

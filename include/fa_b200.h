@@ -280,7 +280,7 @@ int fa_b200_fwd_exchange(const fa_fwd_params* p, void* workspace, size_t workspa
  * KV caches held in 8 bits.  k / v of the cache hold codes, one byte per element, and a scale belongs to every (block of
  * scale_block tokens, kv head) of K and of V: an element stands for code * scale.  scale_block is a multiple of 16 that
  * divides the rows of a page (paged) or of a cache row (contiguous).  Head dims up to 256, multiples of 16; strides of the
- * codes are multiples of 16.
+ * codes are multiples of 16.  Scales are positive or zero, never negative; V's below 2^-64 count as 2^-64.
  * ------------------------------------------------------------------------------------------------ */
 enum fa_code { FA_CODE_E4M3 = 0, FA_CODE_INT8 = 1 };
 typedef struct fa_kv8_cache {

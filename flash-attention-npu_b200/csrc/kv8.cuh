@@ -30,7 +30,8 @@ struct Kv8Params {
   int32_t* status;
 };
 
-// A scale as the kernels use it: zero, or too small to have a reciprocal, stands for nearly nothing; NaN stays NaN.
+// A scale of V as the kernels use it.  Scales are positive, or zero for blocks of zeros: zero, or too small to have a reciprocal, counts as 2^-64;
+// NaN stays NaN.  (K's enter the scores as they are; the tile kernel looks for the maximum before it multiplies by them.)
 __device__ __forceinline__ float usable_scale(float s) { return s < 0x1p-64f ? 0x1p-64f : s; }
 
 // Four codes of a 32-bit word -> two fp16 pairs (bytes 0, 1 and bytes 2, 3); exact.
@@ -56,12 +57,32 @@ struct Kv8Seq {
   const int32_t* pages;            // paged cache
 };
 
+// What the caller's tensors say of a sequence, cut to what there is; fine: nothing had to be cut, and its rows are no more than the caller's
+// longest run, for which there are tiles.
+struct Kv8Lens {
+  int q_row0, q_len, k_len;
+  bool fine;
+};
+__device__ __forceinline__ Kv8Lens kv8_lens(const Kv8Params& p, int bi) {
+  int from = 0, upto = 0, held = 0;  // (all on their way before the first is looked at)
+  if (p.a.cu_seqlens_q) from = p.a.cu_seqlens_q[bi], upto = p.a.cu_seqlens_q[bi + 1];
+  if (p.a.seqused_k) held = p.a.seqused_k[bi];
+  Kv8Lens n{0, p.a.seqlen_q, p.a.seqlen_k + p.a.seqlen_new, true};
+  if (p.a.cu_seqlens_q) n.fine = kv8_query_rows(from, upto, p.a.total_q, n.q_row0, n.q_len) && n.q_len <= p.a.seqlen_q;
+  if (p.a.seqused_k) {
+    const int fits = min(max(held, 0), max(p.a.seqlen_k - p.a.seqlen_new, 0));
+    n.fine &= fits == held;
+    n.k_len = fits + p.a.seqlen_new;
+  }
+  return n;
+}
+
 // The left-window rule needs the longest sequence; warp-collective.
 __device__ __forceinline__ Kv8Mask kv8_mask(const Kv8Params& p, int lane) {
   Kv8Mask m{p.wl, p.wr, false, false};
   if (p.wl_on_device) {
     int mx = 0;
-    for (int i = lane; i < p.a.b; i += 32) mx = max(mx, cache_len(p.a, i, p.status) + p.a.seqlen_new);
+    for (int i = lane; i < p.a.b; i += 32) mx = max(mx, kv8_lens(p, i).k_len);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (mx > 0 && m.wl >= mx - 1) m.wl = -1;
@@ -71,25 +92,14 @@ __device__ __forceinline__ Kv8Mask kv8_mask(const Kv8Params& p, int lane) {
   return m;
 }
 
-// Query rows of a sequence.  Offsets out of range are cut to the rows there are; runs longer than the caller said, of which the tiles cover
-// no more than that, are reported like them.
-__device__ __forceinline__ void kv8_q_rows(const Kv8Params& p, int bi, int& row0, int& len) {
-  row0 = 0;
-  len = p.a.seqlen_q;
-  if (p.a.cu_seqlens_q) {
-    const bool fine = kv8_query_rows(p.a.cu_seqlens_q[bi], p.a.cu_seqlens_q[bi + 1], p.a.total_q, row0, len);
-    if (!fine || len > p.a.seqlen_q) raise_bad_index(p.status);
-  }
-}
-__device__ __forceinline__ int kv8_k_len(const Kv8Params& p, int bi) {
-  return (p.a.seqused_k ? cache_len(p.a, bi, p.status) : p.a.seqlen_k) + p.a.seqlen_new;
-}
-
 // block_m: rows of a tile
 __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Params& p, const Kv8Mask& m, int bi, int mb, int block_m) {
   Kv8Seq s;
-  kv8_q_rows(p, bi, s.q_row0, s.q_len);
-  s.k_len = kv8_k_len(p, bi);
+  const Kv8Lens n = kv8_lens(p, bi);
+  if (!n.fine) raise_bad_index(p.status);  // (here alone: every sequence comes by)
+  s.q_row0 = n.q_row0;
+  s.q_len = n.q_len;
+  s.k_len = n.k_len;
   s.koff = s.k_len - s.q_len;
   const int i_lo = mb * block_m / p.group, i_hi = min(s.q_len, (mb * block_m + block_m - 1) / p.group + 1) - 1;
   kv8_key_range(m, s.k_len, s.koff, i_lo, i_hi, s.key_lo, s.key_hi);
@@ -121,12 +131,10 @@ struct Kv8Walk {
   int bi, nb_lo, nb_hi, n_b, quota, cur, g1, ustart;
 
   __device__ __forceinline__ static void blocks(const Kv8Params& p, const Kv8Mask& m, int bi, int mb, int& nb_lo, int& nb_hi) {
-    int q_row0, q_len;
-    kv8_q_rows(p, bi, q_row0, q_len);
-    const int k_len = kv8_k_len(p, bi);
-    const int i_lo = mb * BM / p.group, i_hi = min(q_len, (mb * BM + BM - 1) / p.group + 1) - 1;
+    const Kv8Lens n = kv8_lens(p, bi);
+    const int i_lo = mb * BM / p.group, i_hi = min(n.q_len, (mb * BM + BM - 1) / p.group + 1) - 1;
     int lo, hi;
-    kv8_key_range(m, k_len, k_len - q_len, i_lo, i_hi, lo, hi);
+    kv8_key_range(m, n.k_len, n.k_len - n.q_len, i_lo, i_hi, lo, hi);
     if (i_hi < i_lo) hi = lo;
     nb_lo = lo / BN;
     nb_hi = hi > lo ? ceil_div(hi, BN) : nb_lo;

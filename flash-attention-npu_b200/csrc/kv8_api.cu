@@ -87,10 +87,10 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
       return fail(FA_ERR_INVALID, "rotary_dim must be divisible by 16 and at most the head dimension");
     if (a.rotary_seqlen < a.seqlen_k) return fail(FA_ERR_INVALID, "rotary_cos / rotary_sin must have a row for every position of the cache");
   }
-  // Rows of a tile and keys of a block are counted in 32 bits.
+  // Rows, keys and window sides: sums and differences of two of them stay within 32 bits (kv8_ranges.cuh).
   const int64_t all_rows = (int64_t)std::max(a.seqlen_q, a.cu_seqlens_q ? a.total_q : 0) * (a.h / a.h_k);
   if (all_rows > 0x3fffffff) return fail(FA_ERR_UNSUPPORTED, "too many query rows in one call");
-  if (a.seqlen_k > 0x7fffffff - 4096) return fail(FA_ERR_UNSUPPORTED, "too many tokens in a sequence's part of the KV cache");
+  if (a.seqlen_k > 1 << 30) return fail(FA_ERR_UNSUPPORTED, "too many tokens in a sequence's part of the KV cache");
   const int rows = a.block_table ? a.page_size : a.seqlen_k;
   const int64_t outer = a.kv_outer > 0 ? a.kv_outer : a.b;
   if (int rc = check_cache(c, rows, a.d); rc != FA_OK) return rc;
@@ -124,8 +124,8 @@ static int make_kv8_plan(const fa_fwd_params& a_in, const fa_kv8_cache& c, Kv8Pl
   }
   bool is_causal = false, is_local = false;
   window_rule(a.seqlen_q, max_k, a.causal != 0, wl, wr, is_causal, is_local);
-  p.wl = std::max(wl, -(1 << 30));  // (sums with positions stay within 32 bits)
-  p.wr = std::max(wr, -(1 << 30));
+  p.wl = std::clamp(wl, -(1 << 30), (1 << 30) - 1);  // (which is as wide as any)
+  p.wr = std::clamp(wr, -(1 << 30), (1 << 30) - 1);
 
   // ---- tile and key splits ----
   const int rows_max = a.seqlen_q * p.group;
@@ -284,7 +284,7 @@ static int run_kvcache_plan(const fa_kvcache_plan_params& p, cudaStream_t st) {
   if (p.b <= 0) return fail(FA_ERR_INVALID, "batch size must be positive");
   if (p.b > FA_B200_PLAN_MAX_REQUESTS)
     return fail(FA_ERR_UNSUPPORTED, "a step has at most " + std::to_string(FA_B200_PLAN_MAX_REQUESTS) + " requests");
-  if (p.page_size <= 0 || p.cols < 0 || p.n_free < 0 || p.total < 0 || p.total > 0x7fffffffLL)
+  if (p.page_size <= 0 || p.cols < 0 || p.n_free < 0 || p.total < 0 || p.total >= 0x7fffffffLL)
     return fail(FA_ERR_INVALID, "bad sizes of the page table, the free list or the packed batch");
   if ((int64_t)p.cols * p.page_size > 0x7fffffffLL) return fail(FA_ERR_UNSUPPORTED, "a row of the page table covers too many tokens");
   if (!p.have || !p.add || (!p.table && p.cols) || (!p.free_pages && p.n_free) || ((!p.slots || !p.positions) && p.total) || !p.cu_new || !p.after ||

@@ -26,15 +26,16 @@ struct Kv8Mask {
 };
 
 // Keys [lo, hi) of the k_len that the query tokens i_lo .. i_hi of a sequence see; none: an empty range within them.  (A range behind
-// the last key had the page table read there, and the scales of blocks that nobody has written.)
+// the last key had the page table read there, and the scales of blocks that nobody has written.)  Within 32 bits: the planner holds keys and
+// rows to 2^30, and the sides of a window to [-2^30, 2^30).
 FA_KV8_HD void kv8_key_range(const Kv8Mask& m, int k_len, int koff, int i_lo, int i_hi, int& lo, int& hi) {
   lo = 0;
   hi = k_len;
   if (m.causal && i_hi + koff + 1 < hi) hi = i_hi + koff + 1;
   if (m.local) {
-    const int64_t first = (int64_t)i_lo + koff - m.wl, behind = (int64_t)i_hi + koff + m.wr + 1;
-    lo = first < 0 ? 0 : first > k_len ? k_len : (int)first;
-    hi = behind > k_len ? k_len : behind < lo ? lo : (int)behind;
+    const int first = i_lo + koff - m.wl, behind = i_hi + koff + m.wr + 1;
+    lo = first < 0 ? 0 : first > k_len ? k_len : first;
+    hi = behind > k_len ? k_len : behind;
   }
   if (hi < lo) hi = lo;
 }

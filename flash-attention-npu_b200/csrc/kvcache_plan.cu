@@ -82,10 +82,10 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
 
   int n_free = p.n_free;
   if (p.num_free) n_free = min(max(*p.num_free, 0), p.n_free);
-  auto behind = [&](const PlanRequest& q, int r) { return q.add > 0 && s_pre[r].x + q.add > p.total; };  // of the packed batch's rows
-  auto granted = [&](const PlanRequest& q, int r) {
-    return q.fits && !behind(q, r) && (q.need == 0 || (int64_t)s_pre[r].y + q.need <= n_free);
-  };
+  auto behind = [&](const PlanRequest& q, int r) { return s_pre[r + 1].x > (int)p.total && q.add > 0; };
+  // (32 bits without a sign hold a sum of two numbers of 31)
+  auto pages_left = [&](const PlanRequest& q, int r) { return q.need == 0 || (uint32_t)s_pre[r].y + (uint32_t)q.need <= (uint32_t)n_free; };
+  auto granted = [&](const PlanRequest& q, int r) { return q.fits && pages_left(q, r) && !behind(q, r); };
   // requests: a warp each
   const int warps = gridDim.x * (kPlanThreads / 32), gw = blockIdx.x * (kPlanThreads / 32) + warp;
   for (int r = gw; r < p.b; r += warps) {
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
     const bool ok = granted(q, r);
     if (lane == 0) {
       p.after[r] = (int)(ok ? q.have + q.add : p.have[r]);
-      p.cu_new[r] = (int)min((int64_t)s_pre[r].x, p.total);
+      p.cu_new[r] = min(s_pre[r].x, (int)p.total);
       if (q.have < 0 || p.add[r] < 0 || behind(q, r)) raise_bad_index(status);
     }
     if (ok)
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
     __syncthreads();
     if (tid == 0) {
       *p.pages_taken = s_pages;
-      p.cu_new[p.b] = (int)min((int64_t)s_pre[p.b].x, p.total);
+      p.cu_new[p.b] = min(s_pre[p.b].x, (int)p.total);
     }
   }
   // tokens
@@ -118,16 +118,16 @@ __global__ void __launch_bounds__(kPlanThreads) kvcache_plan_kernel(const __grid
     int64_t slot = -1;
     int pos = 0;
     if (t < last) {
-      int lo = 0, hi = p.b;  // the last request that starts at or in front of t (empty ones start where the next does)
+      int lo = 0, hi = p.b, end = last;  // the last request that starts at or in front of t (empty ones start where the next does), and its end
       while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_pre[mid].x <= t) lo = mid;
-        else hi = mid;
+        const int mid = (lo + hi) >> 1, at_mid = s_pre[mid].x;
+        if (at_mid <= t) lo = mid;
+        else hi = mid, end = at_mid;
       }
       const PlanRequest q = plan_request(p, lo);
       const int64_t at = q.have + (t - s_pre[lo].x);
       pos = (int)at;
-      if (granted(q, lo) && at >= 0 && at < q.have + q.add) {
+      if (end <= (int)p.total && q.fits && pages_left(q, lo) && at >= 0 && at < q.have + q.add) {
         const int col = (int)((uint32_t)at / (uint32_t)p.page_size), in = (int)at - col * p.page_size;
         const int page = col < q.had ? p.table[(int64_t)lo * p.table_stride + col] : p.free_pages[s_pre[lo].y + col - q.had];
         slot = (int64_t)page * p.page_size + in;

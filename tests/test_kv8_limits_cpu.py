@@ -151,6 +151,7 @@ int any() {
     default: return (int)rng();
   }
 }
+int held(int side) { return side < -(1 << 30) ? -(1 << 30) : side > (1 << 30) - 1 ? (1 << 30) - 1 : side; }
 int some() { return any() & std::numeric_limits<int>::max(); }
 """
 
@@ -193,8 +194,8 @@ int main() {
     const int kind = (int)(rng() % 3);
     m.causal = kind == 1;
     m.local = kind == 2;
-    m.wl = wild ? any() : (int)(rng() % 24) - 6;
-    m.wr = m.causal ? 0 : wild ? any() : (int)(rng() % 24) - 6;
+    m.wl = wild ? held(any()) : (int)(rng() % 24) - 6;
+    m.wr = m.causal ? 0 : wild ? held(any()) : (int)(rng() % 24) - 6;
     const int i_lo = (int)(rng() % q_len), i_hi = i_lo + (int)(rng() % (q_len - i_lo)), koff = k_len - q_len;
     int lo, hi;
     fa::kv8_key_range(m, k_len, koff, i_lo, i_hi, lo, hi);

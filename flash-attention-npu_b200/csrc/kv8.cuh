@@ -113,7 +113,8 @@ __device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Params& p, const Kv8Mask& m, 
 // ---- the work list of a CTA ----
 // A unit is a row tile of one (sequence, kv head).  One unit (or one of its key splits) per CTA, or resident CTAs with equal
 // shares of all units' key blocks: gridDim.x / h_k CTAs a kv head, head fastest, so that the heads of a token, which are neighbours in memory,
-// are read at the same time (8 sequences of 131072 keys, 8 heads of 128 bytes: 313 us, 402 with one unit after the other).  A head's units are
+// are read at the same time (8 sequences of 131072 keys, 8 heads of 128 bytes, calls in a CUDA graph: 313 us, 402 with one unit after
+// the other).  A head's units are
 // laid end to end, each as its key blocks (one, fully masked, when it sees no key, so that its rows are written) behind OVH
 // virtual blocks that stand for its fixed cost; CTA c of the head takes virtual blocks [c * quota, (c + 1) * quota).  A unit that
 // CTA boundaries cut leaves one partial per CTA in consecutive slots.  Producer and consumer warps walk the list independently of one

@@ -5,10 +5,12 @@
 // (K and V) with tiled TMA loads into a ring, and the stage's scales with 4-byte asynchronous copies; consumer warps own 8 or 16 query
 // rows and a slice of the stage's keys each, turn codes into fp16 in registers and multiply with mma.sync (the tile kernel on such calls:
 // 2.2 times as long for 8 rows, 7 % longer for 32; its 128-row tensor instruction waits for the turning of codes all the same).
-// 8 sequences of 131072 keys, 64 / 8 heads of 128: 313 us, 6.85 TB/s.  64 ragged ones of up to 8191 keys with a token appended: 109 us, 5.6
-// TB/s.  32 sequences with a window of 4096 keys and 4 tokens, 64 / 8 heads: 124 us of 40 that HBM would take -- at 32 rows a warp scheduler
-// holds three warps of 168 registers, and what they wait for is one another's products and the instruction cache, not memory (ncu: issue 37
-// %, mma 25 %); eight key slices of 32 rows each, with every code turned once, spill and took 205 us.
+// Calls in a CUDA graph: 8 sequences of 131072 keys, 64 / 8 heads of 128, 315 us, 6.8 TB/s (by themselves, between other kernels' writes, 341 -
+// 371).  64 ragged ones of up to 8191 keys with a token appended: 108 us, 5.6 TB/s.  32 sequences with a window of 4096 keys and 4 tokens,
+// 64 / 8 heads: 123 us of 40 that HBM would take -- at 32 rows a warp scheduler holds three warps of 168 registers, and what they wait for is
+// one another's products and the instruction cache, not memory (ncu: issue 37 %, mma 25 %).  Eight key slices of 32 rows each, with every code
+// turned once, spill and took 205 us; the forms here spill too: 204 bytes a thread at 32 rows of 128 columns and 156 at 16 (168 registers), 280 at
+// 32 rows of 64 (two CTAs, 96 registers), 220 - 360 at 256 columns.
 //
 // Arithmetic.  K = ck * sk(block), V = cv * sv(block).  With the running maximum over x_j = scale * log2e * sk * (q . ck_j) + log2 sv,
 //   P'_j = 2^(x_j - m + 15),   O = sum_j P'_j cv_j / l,   l = sum_j P'_j / sv_j,   LSE = ln2 (m - 15) + ln l:

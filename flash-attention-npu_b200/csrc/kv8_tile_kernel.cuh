@@ -22,11 +22,11 @@
 // TMA cannot convert, so the codes pass through registers: copied ahead into shared memory as they are, read back by the thread that asked
 // for them, turned and stored again.
 //
-// Bound: four chunks of 301 - 2048 tokens against 1777 - 8192 keys, 32 / 8 heads of 128: 485 us, 880 TFLOP/s of what the masks leave.  Per 64
+// Bound: four chunks of 301 - 2048 tokens against 1777 - 8192 keys, 32 / 8 heads of 128: 490 us in a CUDA graph, 870 TFLOP/s of what the masks leave.  Per 64
 // keys and 256 rows a CTA takes 2400 cycles; the products take 1024 of them on the tensor pipe, the exponentials 1024 on the special-function
 // unit, shared memory is busy for 750.  What is left is the chain of one softmax warp (poll, TMEM load, maximum, exponentials, TMEM store,
-// fence) with two such warps a scheduler, as many as registers allow: without any exponential it still takes 1950.  Tried and without
-// gain: a quarter of the exponentials as polynomials (485), a look at the next block's barriers ahead of time (515 - 535), blocks of 128 keys
+// fence) with two such warps a scheduler, as many as registers allow: without any exponential it still takes 1950.  Tried against 485 us
+// and without gain: a quarter of the exponentials as polynomials (485), a look at the next block's barriers ahead of time (515 - 535), blocks of 128 keys
 // with P through shared memory (636).
 #pragma once
 

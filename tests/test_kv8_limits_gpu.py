@@ -181,6 +181,27 @@ def test_a_page_that_is_not_there_holds_nothing(bad, s_q):
         U.check_attention(out[r], lse[r], U.attend(q[r], kv, kv, 2.0 ** -12), tag=f"sequence {r}")
 
 
+@pytest.mark.parametrize("s_q", [1, 40])
+@pytest.mark.parametrize("bad", [4, -1, 2 ** 31 - 1])
+def test_cache_rows_out_of_range(bad, s_q):
+    """A sequence whose cache row is not there gets no token and is reported; the others are what they are without it."""
+    g = _gen(55)
+    kc, ks = _random_cache(g, 4, 96, 2, 64, 3, INT8)
+    rows, lens = [2, bad, 1], [60, 33, 95]
+    x, q = torch.randn((3, 1, 2, 64), generator=g).to(FP), torch.randn((3, s_q, 4, 64), generator=g).to(FP)
+    got, scale = [kc.cuda(), kc.cuda(), ks.cuda(), ks.cuda()], 2.0 ** -12  # (the codes are any)
+    out, lse, *_ = fa3.flash_attn_with_kvcache(q.cuda(), *got[:2], x.cuda(), x.cuda(), cache_seqlens=_i32(lens), cache_batch_idx=_i32(rows),
+                                               k_descale=got[2], v_descale=got[3], softmax_scale=scale, causal=True, return_softmax_lse=True)
+    assert _reported()
+    for r in (0, 2):
+        U.append(x[r], kc, ks, [rows[r] * 96 + lens[r]])
+    for c, s in (got[0::2], got[1::2]):
+        assert torch.equal(s.cpu(), ks) and torch.equal(c.cpu(), kc)
+    for r in (0, 2):
+        kv = torch.stack([U.values_of(kc[rows[r], t]) * ks[rows[r], t // 32].double()[:, None] for t in range(lens[r] + 1)])
+        U.check_attention(out[r], lse[r], U.attend(q[r], kv, kv, scale, True), tag=f"sequence {r}")
+
+
 @pytest.mark.parametrize("s_q", [1, 40, 200])
 def test_lengths_out_of_range(s_q):
     """A length beyond the cache counts as all of it, a negative one as none; both are reported."""

@@ -15,7 +15,8 @@
 // Arithmetic.  K = ck * sk(block), V = cv * sv(block).  With the running maximum over x_j = scale * log2e * sk * (q . ck_j) + log2 sv,
 //   P'_j = 2^(x_j - m + 15),   O = sum_j P'_j cv_j / l,   l = sum_j P'_j / sv_j,   LSE = ln2 (m - 15) + ln l:
 // V's scale rides in the exponent, so that no product is scaled and P' spans all of fp16 (up to 2^15) where what it is multiplied
-// with is largest.  P' is rounded to fp16 (2^-12) for the second product, which is what a 16-bit output can show; the codes
+// with is largest.  P' is rounded to fp16 (2^-12) for the second product, which is what a 16-bit output can show; below 2^-14 (2^-29 of the
+// largest) it is a subnormal, off by 2^-25 at most, that is by 2^-40 of the row's largest weight times scale for each code.  The codes
 // are fp16 values, sums and statistics are fp32.
 //
 // Both products are transposed, S^T = K Q^T and O^T = V^T P^T: query rows are the narrow side of mma m16n8k16, so that the eight rows

@@ -5,7 +5,7 @@
 // among resident CTAs, as the decode kernel does (Kv8Walk).
 // Arithmetic as in kv8_decode_kernel.cuh: V's scale in the exponent, P' in fp16, scales never in a product.  The reference m of
 // the exponent is the running maximum, moved only when that has grown by more than 2^8: P' = 2^(x - m + 7) stays below 2^15, far from
-// fp16's end, and below 2^7 it has as many bits as a 16-bit output shows; so O is rescaled in TMEM a few times a tile and
+// fp16's end, and below 2^7 it has as many bits as a 16-bit output shows (subnormals: off by 2^-32 of the largest at most); so O is rescaled in TMEM a few times a tile and
 // not at every block.
 //
 // Warps: 4 per sub-tile  softmax, one thread per row (P, rescale of O, epilogue); each loads its rows of Q
